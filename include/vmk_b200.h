@@ -14,8 +14,8 @@
  *     enqueued on `stream` (a cudaStream_t passed as void*).  Calls on different streams are
  *     independent when their workspaces differ.
  *   - `status` (nullable) is a device int32 the kernels OR bits into when a bounded device-side wait
- *     ran out (bit 0) or an out-of-range index was clamped (bit 1).  The caller zeroes it and reads it
- *     back after synchronising.
+ *     ran out (bit 0), an out-of-range index was clamped (bit 1) or a page operation was refused (bit 2).  The
+ *     caller zeroes it and reads it back after synchronising.
  *   - Return value: VMK_OK or a negative VMK_E_* code; vmk_error_string() names it.  No C++
  *     exception crosses the boundary.
  */
@@ -260,6 +260,30 @@ VMK_API int vmk_dsa_indexer_hist_fp8(const void* iq8, const float* iq_scale, con
  * applies any to its index queries, are the caller's to apply between the two calls. */
 VMK_API int vmk_dsa_index_project(const void* x, const void* wq, const void* ww, float w_scale, void* iq_out,
                                   float* w_out, int B, int Dx, int bf16, int32_t* status, void* stream);
+
+/* ---- prompt: attention of whole prompts ---------------------------------------------------------------
+ * What fills a cache before the decode ops above read it; the reference has decode ops only (its nearest is the masked
+ * multi-row op, kernels/spec_opus55_v7.py:467-521).  Packed sequences of different lengths, causal, grouped heads:
+ *   q (Tq,Hq,D)  k,v (Tk,Hkv,D)  out (Tq,Hq,D), fp16 (bf16 = 0) or bf16 (1); D must be 128, Hq / Hkv <= 16.
+ *   cu_q, cu_k (S+1) int32 ascending: sequence s has the queries [cu_q[s], cu_q[s+1]) (nq of them) and the keys
+ *   [cu_k[s], cu_k[s+1]) (nk).  causal = 1: query i of a sequence sees its keys j <= nk - nq + i (aligned at the end,
+ *   so that a chunk of new tokens sees the context before it); causal = 0: all nk.  A query that sees no key gets
+ *   zeros, and so do the rows of out outside [cu_q[0], cu_q[S]).  Entries outside their tensor are clamped (status).
+ *   strides (6 int64 in HOST memory, nullable): token and head strides in elements of q, k and v (the innermost axis
+ *   is contiguous); positive multiples of 8.  Null: C-contiguous.  out is C-contiguous.
+ *   Keys of other sequences and behind the last one may hold anything.  A NaN or infinity in v INSIDE a sequence
+ *   reaches the rows that see it, and may reach rows before it whose last block of 128 keys holds it.
+ * vmk_prompt_paged reads the keys of sequence s from the pages of page_table[s] as vmk_decode_paged does: k_pages,
+ * v_pages (pages,Hkv,page_size,D), page_size a multiple of 64, lens (S) int32 = nk (the new tokens included);
+ * strides holds the two of q.  A page id outside [0, pages) reads as zeros. */
+VMK_API size_t vmk_prompt_workspace_bytes(int S, int Tq, int Hq, int Hkv, int D);
+VMK_API int vmk_prompt(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
+                       const int64_t* strides, void* out, int S, int Tq, int Tk, int Hq, int Hkv, int D, int causal,
+                       int bf16, void* ws, size_t ws_bytes, int32_t* status, void* stream);
+VMK_API int vmk_prompt_paged(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
+                             int pages, int page_size, int table_stride, const int32_t* cu_q, const int32_t* lens,
+                             const int64_t* strides, void* out, int S, int Tq, int Hq, int Hkv, int D, int causal,
+                             int bf16, void* ws, size_t ws_bytes, int32_t* status, void* stream);
 
 /* ---- merge of split partials -------------------------------------------------------------------
  * Log-sum-exp merge used after a KV split across GPUs (the reference merges its in-GPU splits the

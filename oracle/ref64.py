@@ -161,3 +161,31 @@ def decode_ref64(q, k, v, lens, **_):
             s = (qb[h] @ k[b, h, :n].T) / np.sqrt(D)
             out[b, h * G:(h + 1) * G] = _softmax_rows_times(s, v[b, h, :n])
     return out
+
+
+def prompt_ref64(q, k, v, nq, nk, causal=True):
+    """Attention of packed prompts (no counterpart in the reference, whose ops decode; the arithmetic is that of
+    spec_ref64, ops/spec.py:69-82, with a causal mask aligned at the end).  q (Tq,Hq,D); k, v (Tk,Hkv,D); nq, nk: the
+    queries and keys of each sequence, packed one after the other from row 0.  Returns (out, a, s), each float64: the
+    output (zeros where a query sees no key and behind the last sequence), and per output row what error bounds need:
+    a (Tq,Hq,D) = sum_j p_j |v_j| and s (Tq,Hq) = the largest sum_d |q_d k_d| / sqrt(D) over the keys it sees."""
+    q, k, v = _f64(q), _f64(k), _f64(v)
+    Tq, Hq, D = q.shape
+    G = Hq // k.shape[1]
+    out, a, s = np.zeros((Tq, Hq, D)), np.zeros((Tq, Hq, D)), np.zeros((Tq, Hq))
+    tq = tk = 0
+    for n, m in zip(nq, nk):
+        for h in range(Hq):
+            kk, vv = k[tk:tk + m, h // G], v[tk:tk + m, h // G]
+            for i in range(n):
+                c = min(m, max(0, m - n + i + 1)) if causal else m
+                if c == 0:
+                    continue
+                with np.errstate(invalid="ignore", over="ignore"):
+                    x = kk[:c] @ q[tq + i, h] / math.sqrt(D)
+                    p = np.exp(x - x.max())
+                    p /= p.sum()
+                    out[tq + i, h], a[tq + i, h] = p @ vv[:c], p @ np.abs(vv[:c])
+                    s[tq + i, h] = (np.abs(kk[:c]) @ np.abs(q[tq + i, h])).max() / math.sqrt(D)
+        tq, tk = tq + n, tk + m
+    return out, a, s

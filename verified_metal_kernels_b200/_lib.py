@@ -43,6 +43,9 @@ SIGNATURES = {
     "vmk_dsa_attend_bf16": (_i, [_vp] * 5 + [_i] * 2 + [_vp, _sz, _vp, _vp]),
     "vmk_dsa_gather": (_i, [_vp] * 5 + [_i] * 2 + [_vp, _vp]),
     "vmk_dsa_index_project": (_i, [_vp] * 3 + [_c.c_float] + [_vp] * 2 + [_i] * 3 + [_vp, _vp]),
+    "vmk_prompt_workspace_bytes": (_sz, [_i] * 5),
+    "vmk_prompt": (_i, [_vp] * 7 + [_i] * 8 + [_vp, _sz, _vp, _vp]),
+    "vmk_prompt_paged": (_i, [_vp] * 4 + [_i] * 3 + [_vp] * 4 + [_i] * 7 + [_vp, _sz, _vp, _vp]),
     "vmk_lse_merge": (_i, [_vp] * 3 + [_i] * 3 + [_vp, _vp]),
     "vmk_prefix_partial": (_i, [_vp] * 6 + [_i] * 9 + [_vp] * 3 + [_vp, _sz, _vp, _vp]),
     "vmk_spec_partial": (_i, [_vp] * 4 + [_i] + [_i] * 8 + [_vp] * 3 + [_vp, _sz, _vp, _vp]),
@@ -70,12 +73,13 @@ class VmkError(RuntimeError):
 class VmkDeviceStatusError(VmkError):
     """The device status word was non-zero after a call: bit 0 = a bounded device-side wait ran out (the CTA that
     gave up wrote no result, so the WHOLE call's output is invalid), bit 1 = an index or length outside its tensor
-    was clamped."""
+    was clamped, bit 2 = a page operation was refused."""
 
     def __init__(self, status, what):
         self.code, self.status = None, status
         bits = [n for b, n in ((1, "a bounded device-side wait ran out: the output is invalid"),
-                               (2, "an out-of-range index or length was clamped")) if status & b]
+                               (2, "an out-of-range index or length was clamped"),
+                               (4, "a page operation was refused: no free page left, or a page that others share")) if status & b]
         RuntimeError.__init__(self, f"{what}: device status word {status} ({'; '.join(bits) or 'unknown bits'})")
 
 
@@ -126,6 +130,13 @@ class Workspace:
 
 _workspace = Workspace()
 _status = {}
+
+
+def scratch(nbytes, device):
+    """Scratch of one call, from torch's allocator on the current stream: a captured graph keeps its own, and a call
+    on another stream has another."""
+    import torch
+    return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
 
 
 def workspace(nbytes, device, stream_id):

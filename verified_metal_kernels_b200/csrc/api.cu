@@ -64,6 +64,27 @@ int make_tmap_rows(CUtensorMap* tm, const void* base, uint64_t width, uint64_t r
   return r == CUDA_SUCCESS ? VMK_OK : VMK_E_DRIVER;
 }
 
+int make_tmap_strided(CUtensorMap* tm, const void* base, uint64_t heads, uint64_t tokens, int64_t head_stride,
+                      int64_t token_stride, uint32_t box_w, uint32_t box_heads, uint32_t box_tokens) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return VMK_E_DRIVER;
+  // the stride of an axis of length one is never used: give it a value that the encoder takes
+  if (heads == 1) head_stride = 128;
+  if (tokens == 1) token_stride = 128;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) != 0 || head_stride <= 0 || token_stride <= 0 || head_stride % 8 != 0 ||
+      token_stride % 8 != 0 || head_stride >= (int64_t(1) << 39) || token_stride >= (int64_t(1) << 39) || box_w * 2 != 128 ||
+      box_heads > 256 || box_tokens > 256)
+    return VMK_E_BADARG;
+  cuuint64_t dims[3] = {128, heads, tokens};
+  cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2};
+  cuuint32_t box[3] = {box_w, box_heads, box_tokens};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? VMK_OK : VMK_E_DRIVER;
+}
+
 // The same for a tensor of bytes (fp8): (groups, rows, 128) with one 128-byte swizzled row per tensor row.
 int make_tmap_3d_u8(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t groups, uint32_t box_rows) {
   auto fn = encode_fn();

@@ -17,6 +17,7 @@ constexpr uint32_t kSpinLimit = 1u << 22;   // bound on every mbarrier wait; exc
 // Bits of the device status word (written with atomicOr; 0 means clean).
 constexpr int kStatusTimeout = 1;     // a bounded wait ran out
 constexpr int kStatusBadIndex = 2;    // an index outside its tensor was clamped
+constexpr int kStatusPages = 4;       // a page operation was refused: no free page left, or a page that is shared
 
 // ------------------------------------------------------------------------------------------------
 // shared-memory addresses, mbarrier
@@ -223,6 +224,10 @@ constexpr int kSelShift = 21;
 // Returns 0 or a VMK_E_* code.
 int make_tmap_3d(CUtensorMap* tm, const void* base, uint64_t width, uint64_t rows, uint64_t groups,
                  uint32_t box_w, uint32_t box_rows);
+// The same over a tensor of 16-bit values viewed as (tokens, heads, 128) with any strides (in elements, positive multiples
+// of 8): box = (64, box_heads, box_tokens).
+int make_tmap_strided(CUtensorMap* tm, const void* base, uint64_t heads, uint64_t tokens, int64_t head_stride,
+                      int64_t token_stride, uint32_t box_w, uint32_t box_heads, uint32_t box_tokens);
 int make_tmap_3d_u8(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t groups, uint32_t box_rows);
 
 int sm_count();

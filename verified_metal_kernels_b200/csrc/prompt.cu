@@ -1,0 +1,769 @@
+// Attention of whole prompts (or of chunks of prompts over a cache) on the 5th-generation tensor cores: what fills a
+// serving engine before the decode kernels of this library take over.  The reference defines decode ops only; the
+// float64 statement lives in oracle/ref64.py (prompt_ref64).
+//
+//   sequence s has the queries [cu_q[s], cu_q[s+1]) (nq of them) and nk keys; query i of it sees the keys
+//   j <= nk - nq + i (causal, aligned at the end) or all nk of them:
+//       out[i] = sum_j exp(q_i . k_j / sqrt(128) - m_i) v_j / sum_j exp(q_i . k_j / sqrt(128) - m_i)
+//   in one pass over the keys with the running maximum m and sum of the softmax in fp32; a query that sees no key
+//   gets zeros, and so do rows of `out` outside every sequence.
+//
+// One UNIT of work = (256-row tile of a sequence, kv head): the rows of a tile are stacked (token, query head of the
+// group) pairs, so every K/V tile is read once for the whole group; the tile is two 128-row tiles A and B that share
+// the K/V tiles and alternate on the tensor pipe.  A group of G heads puts floor(128 / G) tokens into a tile (the
+// rest of its rows is unused).  A planner kernel (one CTA) lists the tiles of all sequences, those with the most key
+// blocks first (under a causal mask the last tile of a prompt costs many times its first, and units are handed out
+// in that order by an atomic counter, so the short ones fill the end), and a PERSISTENT CTA per SM takes units.
+// 384 threads, warp-specialised:
+//   warp 8      takes units from the counter, hands them to the other warps through a two-entry ring, and is the TMA
+//               producer: Q tiles, and K_0, V_0, K_1, V_1, ... into one ring of five 32 KiB slots, running ahead into
+//               the next unit
+//   warp 9      owns tensor memory and issues every tcgen05.mma, in the order  P.V of tile t at block j, then Q.K^T of
+//               tile t at block j + 1, tiles alternating.  Products of one thread execute in order, so Q.K^T may
+//               overwrite the scores of a block as soon as the P.V that reads their P is issued: no wait between the
+//               two, and the pipe runs one tile's pair while the other tile's softmax works
+//   warps 0-3   softmax of tile A, warps 4-7 of tile B: one thread per row
+//   warp 10     zeroes the rows of `out` outside every sequence (warp 11 only completes the warp group)
+// Tensor memory (512 columns): S_A, S_B, O_A, O_B, 128 columns each; P (16-bit pairs, 64 columns) over its scores.
+// O is rescaled only when a row's maximum grew by more than 2^8 (P stays below 2^8 and the result is exact); the
+// softmax thread does it itself: when the scores of block j are there, the P.V of block j - 1, issued before them,
+// has completed.  P is rounded to the tensors' 16-bit type before P.V (the tensor pipe takes 16-bit operands); the
+// sum that divides is that of the unrounded P.
+//
+// Rows of V past the end of a sequence (the next sequence's, or whatever a page holds there) are cleared in shared
+// memory before the product: their P is 0, but 0 times Inf would poison the row.
+// Every mbarrier wait is bounded; a wait that runs out sets the status word and the CTA winds down through the common
+// exit, where tensor memory is freed.
+#include <atomic>
+#include <cstring>
+#include <type_traits>
+
+#include "tcgen05.cuh"
+
+namespace vmk {
+
+constexpr int kPmBK = 128;                       // keys per block
+constexpr int kPmD = 128;
+constexpr int kPmHalf = 128 * 128;               // [128 rows][128 B] swizzled: one 64-wide half of the head dim
+constexpr int kPmTile = 2 * kPmHalf;             // 32 KiB: a Q, K or V tile
+constexpr int kPmSlots = 5;
+constexpr int kPmSched = 2;
+constexpr int kPmThreads = 384;                // 12 warps x 168 registers; after set-up 2 x 128 threads hold 216, 128 hold 72
+constexpr int kPmCols = 512;
+constexpr int kPmColS = 0, kPmColO = 256;
+constexpr float kPmLazy = 8.f;                   // log2 units
+constexpr int kPmPlanThreads = 1024;
+constexpr int kPmBins = 256;
+
+struct PromptItem {          // one 256-row tile of one sequence
+  int tok0;                  // first query token (index into q)
+  int ntok;                  // tokens of the tile, 1 .. 2 * tokens per 128-row tile
+  int k0;                    // contiguous keys: index of the sequence's first key; paged: the sequence
+  int nk;                    // keys of the sequence
+  int vis0;                  // keys the tile's first token sees, minus one; token i sees min(nk, vis0 + i + 1)
+  int pad[3];
+};
+
+struct PromptCtrl {
+  int n_items;
+  int next;                  // next unit to hand out
+  int q_lo, q_hi;            // rows of q inside sequences: [q_lo, q_hi)
+};
+
+struct PromptParams {
+  CUtensorMap tmQ, tmK, tmV;
+  __half* out;
+  const PromptItem* items;
+  PromptCtrl* ctrl;
+  const int32_t* page_table;   // paged cache: (S, table_stride); null = packed keys
+  int page_size, table_stride, page_groups;
+  int Tq, Hq, Hkv, G, tpt;     // tpt = tokens per 128-row tile
+  float sc;                    // log2(e) / sqrt(128)
+  int bf16;
+  int32_t* status;
+};
+
+struct PromptPlanParams {
+  const int32_t *cu_q, *cu_k, *lens;   // lens: paged (keys of each sequence); else cu_k
+  PromptItem* items;
+  PromptCtrl* ctrl;
+  int S, Tq, Tk, tpt, causal, max_items, first_units;
+  int32_t* status;
+};
+
+// Blocks of keys -> 0 .. 255, growing: exact below 16, then four bits of mantissa.
+__device__ __forceinline__ int cost_bin(int nblk) {
+  if (nblk < 16) return nblk;
+  const int e = 31 - __clz(nblk);
+  return min(kPmBins - 1, 16 + (e - 4) * 16 + ((nblk >> (e - 4)) & 15));
+}
+
+// One sequence's queries and keys, clamped into their tensors.
+__device__ __forceinline__ bool prompt_seq(const PromptPlanParams& p, int s, int& q0, int& nq, int& k0, int& nk) {
+  bool bad = false;
+  auto inside = [&](int v, int hi) {
+    if (v < 0 || v > hi) bad = true;
+    return min(max(v, 0), hi);
+  };
+  q0 = inside(p.cu_q[s], p.Tq);
+  nq = inside(p.cu_q[s + 1], p.Tq) - q0;
+  if (p.lens != nullptr) {
+    k0 = s;
+    nk = inside(p.lens[s], p.Tk);
+  } else {
+    k0 = inside(p.cu_k[s], p.Tk);
+    nk = inside(p.cu_k[s + 1], p.Tk) - k0;
+  }
+  if (nq < 0 || nk < 0) bad = true;
+  nq = max(nq, 0);
+  nk = max(nk, 0);
+  return bad;
+}
+
+__global__ void __launch_bounds__(kPmPlanThreads, 1) prompt_plan_kernel(const PromptPlanParams p) {
+  __shared__ int s_start[kPmPlanThreads + 1];
+  __shared__ int s_q0[kPmPlanThreads], s_nq[kPmPlanThreads], s_k0[kPmPlanThreads], s_nk[kPmPlanThreads];
+  __shared__ int s_hist[kPmBins];
+  __shared__ int s_warp[32];
+  __shared__ int s_total;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_release();
+  if (tid < kPmBins) s_hist[tid] = 0;
+  if (tid == 0) s_total = 0;
+  pdl_wait();
+  const int per = 2 * p.tpt;
+  bool bad = false;
+  // Pass 0 counts the tiles of each cost, pass 1 places them, the costly ones first.
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int base = 0; base < p.S; base += kPmPlanThreads) {
+      const int s = base + tid;
+      int q0 = 0, nq = 0, k0 = 0, nk = 0;
+      if (s < p.S) bad |= prompt_seq(p, s, q0, nq, k0, nk);
+      const int tiles = (nq + per - 1) / per;
+      int incl = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      __syncthreads();                          // the chunk before is done with the shared arrays
+      if (lane == 31) s_warp[warp] = incl;
+      __syncthreads();
+      if (warp == 0) {
+        int w = s_warp[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, w, o);
+          if (lane >= o) w += v;
+        }
+        s_warp[lane] = w;
+      }
+      __syncthreads();
+      incl += warp > 0 ? s_warp[warp - 1] : 0;
+      s_start[tid] = incl - tiles;
+      s_q0[tid] = q0;
+      s_nq[tid] = nq;
+      s_k0[tid] = k0;
+      s_nk[tid] = nk;
+      if (tid == kPmPlanThreads - 1) s_start[kPmPlanThreads] = incl;
+      __syncthreads();
+      const int total = s_start[kPmPlanThreads];
+      for (int i = tid; i < total; i += kPmPlanThreads) {
+        int lo = 0, hi = kPmPlanThreads;        // the last sequence whose first tile is at or before i
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (s_start[mid] <= i) lo = mid; else hi = mid;
+        }
+        const int t = i - s_start[lo];
+        PromptItem it;
+        it.tok0 = s_q0[lo] + t * per;
+        it.ntok = min(per, s_nq[lo] - t * per);
+        it.k0 = s_k0[lo];
+        it.nk = s_nk[lo];
+        it.vis0 = p.causal ? it.nk - s_nq[lo] + t * per : it.nk;
+        it.pad[0] = it.pad[1] = it.pad[2] = 0;
+        const int seen = min(it.nk, max(0, it.vis0 + it.ntok));
+        const int bin = kPmBins - 1 - cost_bin((seen + kPmBK - 1) / kPmBK);
+        if (pass == 0) {
+          atomicAdd(&s_hist[bin], 1);
+        } else {
+          const int at = atomicAdd(&s_hist[bin], 1);
+          if (at < p.max_items) p.items[at] = it;
+        }
+      }
+    }
+    __syncthreads();
+    if (pass == 0) {
+      if (warp == 0) {                          // exclusive scan of the 256 bins by one warp
+        int v[kPmBins / 32], sum = 0;
+#pragma unroll
+        for (int i = 0; i < kPmBins / 32; ++i) {
+          v[i] = s_hist[lane * (kPmBins / 32) + i];
+          sum += v[i];
+        }
+        int incl = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += x;
+        }
+        int at = incl - sum;
+#pragma unroll
+        for (int i = 0; i < kPmBins / 32; ++i) {
+          s_hist[lane * (kPmBins / 32) + i] = at;
+          at += v[i];
+        }
+        if (lane == 31) s_total = at;
+      }
+      __syncthreads();
+    }
+  }
+  if (tid == 0) {
+    const int lo = min(max(p.cu_q[0], 0), p.Tq);
+    p.ctrl->n_items = min(s_total, p.max_items);
+    p.ctrl->next = p.first_units;
+    p.ctrl->q_lo = lo;
+    p.ctrl->q_hi = max(lo, min(max(p.cu_q[p.S], 0), p.Tq));
+    if (s_total > p.max_items) bad = true;      // sequences that overlap: more rows than q has
+  }
+  if (bad) report(p.status, kStatusBadIndex);
+}
+
+__device__ __forceinline__ float pm_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct PromptUnit {          // what warp 8 hands to the others
+  PromptItem it;
+  int h;                     // kv head; -1: no more units
+  int pad[3];
+};
+
+// Key blocks that 128-row tile t of an item has to see, and how many tokens it holds.
+__device__ __forceinline__ int tile_blocks(const PromptItem& it, int t, int tpt) {
+  const int tok = min(it.ntok, (t + 1) * tpt);
+  if (tok <= t * tpt) return 0;
+  const int seen = min(it.nk, max(0, it.vis0 + tok));
+  return (seen + kPmBK - 1) / kPmBK;
+}
+
+constexpr int kPmBars = 2 * kPmSlots + 2 * kPmSched + 2 + 2 + 2 + 2 + 2;
+constexpr int kPmSmem = 2 * kPmTile + kPmSlots * kPmTile + kPmBars * 8 + kPmSched * (int)sizeof(PromptUnit) + 16 + 1024;
+static_assert(kPmSmem <= 232448, "shared memory of one CTA");
+
+__global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_constant__ PromptParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;                                    // [2 tiles][32 KiB]
+  uint8_t* sKV = sQ + 2 * kPmTile;                       // [slots][32 KiB]
+  uint64_t* full = reinterpret_cast<uint64_t*>(sKV + kPmSlots * kPmTile);   // K or V tile landed (TMA bytes)
+  uint64_t* empty = full + kPmSlots;                     // consumed by both tiles' products   (MMA commit)
+  uint64_t* sched_full = empty + kPmSlots;               // unit written                       (warp 8)
+  uint64_t* sched_empty = sched_full + kPmSched;         // unit read by everybody             (9 warps)
+  uint64_t* q_full = sched_empty + kPmSched;             // [tile] Q tile landed               (TMA bytes)
+  uint64_t* q_empty = q_full + 2;                        // [tile] last Q.K^T of a unit done   (MMA commit)
+  uint64_t* s_full = q_empty + 2;                        // [tile] scores ready                (MMA commit)
+  uint64_t* p_full = s_full + 2;                         // [tile] P in tensor memory          (4 warps)
+  uint64_t* o_full = p_full + 2;                         // [tile] last P.V of a unit done     (MMA commit)
+  PromptUnit* units = reinterpret_cast<PromptUnit*>(sKV + kPmSlots * kPmTile + kPmBars * 8);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(units + kPmSched);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < kPmSlots; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < kPmSched; ++s) {
+      mbar_init(&sched_full[s], 1);
+      mbar_init(&sched_empty[s], 9);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_full[t], 1);
+      mbar_init(&q_empty[t], 1);
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_full[t], 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 9) tmem_alloc(tmem_slot, kPmCols);
+  if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&p.tmQ);
+    tma_prefetch_desc(&p.tmK);
+    tma_prefetch_desc(&p.tmV);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();
+
+  // The registers of a block are fixed at its launch (384 x 168 = 64512): 256 x 216 + 128 x 72 is the same number.  Each
+  // side changes its share as the first thing in its own branch; the branches meet again only at the common exit.
+  bool timed_out = false;
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  if (warp == 8) {
+    // ------------------------------------------------------------------------------ units and TMA producer
+    if (lane == 0) {
+      const int n_units = p.ctrl->n_items * p.Hkv;
+      const uint32_t q_bytes = (uint32_t)(p.tpt * p.G) * 128u * 2u;
+      int u = blockIdx.x;
+      uint32_t ring = 0, issued_q[2] = {0, 0};
+      for (uint32_t n = 0;; ++n) {
+        const int sl = n % kPmSched;
+        if (n >= kPmSched && !mbar_wait(&sched_empty[sl], (n / kPmSched - 1) & 1)) { timed_out = true; break; }
+        PromptUnit un;
+        un.h = -1;
+        if (u < n_units) {
+          un.it = p.items[u / p.Hkv];
+          un.h = u % p.Hkv;
+        }
+        units[sl].it = un.it;
+        units[sl].h = un.h;
+        mbar_arrive(&sched_full[sl]);
+        if (un.h < 0) break;
+        const int nt0 = tile_blocks(un.it, 0, p.tpt), nt1 = tile_blocks(un.it, 1, p.tpt);
+        const int nblk = max(nt0, nt1);
+        for (int i = 0; i < 2 * nblk; ++i, ++ring) {
+          const int s = ring % kPmSlots;
+          if (ring >= kPmSlots && !mbar_wait(&empty[s], (ring / kPmSlots - 1) & 1)) { timed_out = true; break; }
+          const CUtensorMap* tm = (i & 1) ? &p.tmV : &p.tmK;
+          uint8_t* dst = sKV + s * kPmTile;
+          const int kb = (i >> 1) * kPmBK;
+          mbar_expect_tx(&full[s], kPmTile);
+          if (p.page_table == nullptr) {
+            tma_load_3d(dst, tm, 0, un.h, un.it.k0 + kb, &full[s]);
+            tma_load_3d(dst + kPmHalf, tm, 64, un.h, un.it.k0 + kb, &full[s]);
+          } else {
+            // two 64-key boxes, each inside one page; a page id outside the pool reads zeros
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              const int y = kb + b * 64, pg = y / p.page_size;
+              const int id = pg < p.table_stride ? p.page_table[(size_t)un.it.k0 * p.table_stride + pg] : -1;
+              const int z = (id >= 0 && id < p.page_groups / p.Hkv) ? id * p.Hkv + un.h : p.page_groups;
+              tma_load_3d(dst + b * (kPmHalf / 2), tm, 0, y - pg * p.page_size, z, &full[s]);
+              tma_load_3d(dst + kPmHalf + b * (kPmHalf / 2), tm, 64, y - pg * p.page_size, z, &full[s]);
+            }
+          }
+          if (i == 0) {
+            // the queries behind the first keys: the slot of K_0 is free earlier than the Q tiles of the unit before
+            for (int t = 0; t < 2 && !timed_out; ++t) {
+              if ((t == 0 ? nt0 : nt1) == 0) continue;
+              if (issued_q[t] > 0 && !mbar_wait(&q_empty[t], (issued_q[t] - 1) & 1)) { timed_out = true; break; }
+              ++issued_q[t];
+              mbar_expect_tx(&q_full[t], q_bytes);
+              tma_load_3d(sQ + t * kPmTile, &p.tmQ, 0, un.h * p.G, un.it.tok0 + t * p.tpt, &q_full[t]);
+              tma_load_3d(sQ + t * kPmTile + kPmHalf, &p.tmQ, 64, un.h * p.G, un.it.tok0 + t * p.tpt, &q_full[t]);
+            }
+            if (timed_out) { ++ring; break; }
+          }
+        }
+        if (timed_out) break;
+        u = atomicAdd(&p.ctrl->next, 1);
+      }
+      // no load outlives the CTA: the newest tile of every slot has landed before this warp goes to the exit
+      for (uint32_t i = ring > kPmSlots ? ring - kPmSlots : 0; i < ring; ++i) mbar_wait(&full[i % kPmSlots], (i / kPmSlots) & 1);
+      for (int t = 0; t < 2; ++t)
+        if (issued_q[t] > 0) mbar_wait(&q_full[t], (issued_q[t] - 1) & 1);
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------------------------ every tcgen05.mma
+    if (lane == 0) {
+      const uint32_t idesc_qk = umma_idesc_16(128, kPmBK, 0, p.bf16), idesc_pv = umma_idesc_16(128, kPmD, 1, p.bf16);
+      const uint32_t hi_k = (uint32_t)(umma_desc_sw128(0) >> 32), lo_k = (uint32_t)umma_desc_sw128(0);
+      const uint32_t q_lo = lo_k + (smem_u32(sQ) >> 4), k_lo = lo_k + (smem_u32(sKV) >> 4);
+      const uint32_t hi_v = (uint32_t)(umma_desc_sw128_mn(0, kPmHalf, 1024) >> 32);
+      const uint32_t v_lo = (uint32_t)umma_desc_sw128_mn(0, kPmHalf, 1024) + (smem_u32(sKV) >> 4);
+      uint32_t ring = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
+      auto qk = [&](int t, uint32_t slot) {
+        const uint32_t d = tmem_base + kPmColS + t * 128, a = q_lo + t * (kPmTile >> 4), b = k_lo + slot * (kPmTile >> 4);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          umma_f16_w(d, a + (k >> 2) * (kPmHalf >> 4) + (k & 3) * 2, hi_k, b + (k >> 2) * (kPmHalf >> 4) + (k & 3) * 2, hi_k,
+                     idesc_qk, k > 0 ? 1u : 0u);
+        umma_commit(&s_full[t]);
+      };
+      for (uint32_t n = 0; !timed_out; ++n) {
+        const int sl = n % kPmSched;
+        if (!mbar_wait(&sched_full[sl], (n / kPmSched) & 1)) { timed_out = true; break; }
+        const int h = units[sl].h;
+        int nt[2] = {0, 0};
+        if (h >= 0) {
+          nt[0] = tile_blocks(units[sl].it, 0, p.tpt);
+          nt[1] = tile_blocks(units[sl].it, 1, p.tpt);
+        }
+        mbar_arrive(&sched_empty[sl]);
+        if (h < 0) break;
+        const int nblk = max(nt[0], nt[1]);
+        if (nblk == 0) continue;
+        auto wait_tile = [&](uint32_t i) {
+          if (!mbar_wait(&full[i % kPmSlots], (i / kPmSlots) & 1)) timed_out = true;
+        };
+        wait_tile(ring);                                   // K_0
+        for (int t = 0; t < 2 && !timed_out; ++t) {
+          if (nt[t] == 0) continue;
+          if (!mbar_wait(&q_full[t], n_q[t]++ & 1)) { timed_out = true; break; }
+          tc_fence_after();
+          qk(t, ring % kPmSlots);
+          if (nt[t] == 1) umma_commit(&q_empty[t]);
+        }
+        if (timed_out) break;
+        umma_commit(&empty[ring % kPmSlots]);
+        for (int j = 0; j < nblk && !timed_out; ++j) {
+          const uint32_t iv = ring + 2 * j + 1, ik = iv + 1;
+          wait_tile(iv);
+          if (j + 1 < nblk) wait_tile(ik);
+          if (timed_out) break;
+          for (int t = 0; t < 2; ++t) {
+            if (j >= nt[t]) continue;
+            if (!mbar_wait(&p_full[t], n_p[t]++ & 1)) { timed_out = true; break; }
+            tc_fence_after();
+            const uint32_t o = tmem_base + kPmColO + t * 128, a = tmem_base + kPmColS + t * 128;
+            const uint32_t b = v_lo + (iv % kPmSlots) * (kPmTile >> 4);
+#pragma unroll
+            for (int k = 0; k < kPmBK / 16; ++k) umma_f16_ts(o, a + k * 8, b + k * (2048 >> 4), hi_v, idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
+            if (j + 1 == nt[t]) {
+              umma_commit(&o_full[t]);
+            } else {
+              qk(t, ik % kPmSlots);
+              if (j + 2 == nt[t]) umma_commit(&q_empty[t]);
+            }
+          }
+          if (timed_out) break;
+          umma_commit(&empty[iv % kPmSlots]);
+          if (j + 1 < nblk) umma_commit(&empty[ik % kPmSlots]);
+        }
+        ring += 2 * nblk;
+      }
+    }
+  } else if (warp == 10) {
+    // ------------------------------------------------------------------------------ rows outside every sequence
+    const int lo = p.ctrl->q_lo, hi = p.ctrl->q_hi;
+    const size_t row16 = (size_t)p.Hq * (kPmD / 8);       // 16-byte chunks of one token's row
+    const size_t n = (size_t)(lo + (p.Tq - hi)) * row16;
+    for (size_t e = (size_t)blockIdx.x * 32 + lane; e < n; e += (size_t)gridDim.x * 32) {
+      const size_t at = e < (size_t)lo * row16 ? e : e - (size_t)lo * row16 + (size_t)hi * row16;
+      reinterpret_cast<uint4*>(p.out)[at] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    // ------------------------------------------------------------------------------ softmax
+    const int t = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;               // row of the tile = tensor-memory lane
+    const uint32_t lane_base = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t tS = lane_base + kPmColS + t * 128, tO = lane_base + kPmColO + t * 128;
+    const int tok = row / p.G;                            // token of the row inside its 128-row tile
+    const int g = row - tok * p.G;
+    uint32_t ring = 0, n_s = 0, n_o = 0;
+    for (uint32_t n = 0; !timed_out; ++n) {
+      const int sl = n % kPmSched;
+      if (!__all_sync(0xffffffffu, mbar_wait(&sched_full[sl], (n / kPmSched) & 1))) { timed_out = true; break; }
+      const PromptItem it = units[sl].it;
+      const int h = units[sl].h;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sched_empty[sl]);
+      if (h < 0) break;
+      const int na = tile_blocks(it, 0, p.tpt), nb = tile_blocks(it, 1, p.tpt);
+      const int nblk = max(na, nb), mine = t == 0 ? na : nb;
+      const int tk = t * p.tpt + tok;                     // token of the row inside the item
+      const bool valid = tok < p.tpt && tk < it.ntok;
+      const int vis = valid ? min(it.nk, max(0, it.vis0 + tk + 1)) : 0;
+      // keys that every row of this tile sees (its first token's)
+      const int vis_all = min(it.nk, max(0, it.vis0 + t * p.tpt + 1));
+
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < mine; ++j) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], n_s++ & 1))) { timed_out = true; break; }
+        tc_fence_after();
+        const int kb = j * kPmBK;
+        uint32_t s0[32], s1[32], s2[32], s3[32];
+        tmem_ld32(tS, s0);
+        tmem_ld32(tS + 32, s1);
+        tmem_ld32(tS + 64, s2);
+        tmem_ld32(tS + 96, s3);
+        tmem_ld_wait();
+        if (kb + kPmBK > vis_all) {
+          // a block that the mask or the end of the keys cuts: hidden scores become -inf whatever they were
+          const int lim = vis - kb;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (i >= lim) s0[i] = 0xff800000u;
+            if (i + 32 >= lim) s1[i] = 0xff800000u;
+            if (i + 64 >= lim) s2[i] = 0xff800000u;
+            if (i + 96 >= lim) s3[i] = 0xff800000u;
+          }
+        }
+        float b0 = -INFINITY, b1 = -INFINITY, b2 = -INFINITY, b3 = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          b0 = fmaxf(b0, __uint_as_float(s0[i]));
+          b1 = fmaxf(b1, __uint_as_float(s1[i]));
+          b2 = fmaxf(b2, __uint_as_float(s2[i]));
+          b3 = fmaxf(b3, __uint_as_float(s3[i]));
+        }
+        const float bm = fmaxf(fmaxf(b0, b1), fmaxf(b2, b3)) * p.sc;      // the scale is positive: max commutes with it
+        const float m_new = fmaxf(m, bm);
+        float alpha = 1.f;
+        bool rescale = false;
+        if (m == -INFINITY) {
+          m = m_new;                                     // nothing accumulated for this row yet
+        } else if (m_new > m + kPmLazy) {
+          alpha = pm_exp2(m - m_new);
+          m = m_new;
+          rescale = true;
+        }
+        l *= alpha;
+        const float mu = (m == -INFINITY) ? 0.f : m;
+        if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {
+            uint32_t o[16];
+            tmem_ld16(tO + c * 16, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st16(tO + c * 16, o);
+          }
+        }
+        float ps0 = 0.f, ps1 = 0.f;
+        auto to_p = [&](auto bf_tag, uint32_t (&sc32)[32], int c) {
+          constexpr bool BF = decltype(bf_tag)::value;
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float a = pm_exp2(fmaf(__uint_as_float(sc32[i]), p.sc, -mu));
+            const float b = pm_exp2(fmaf(__uint_as_float(sc32[i + 1]), p.sc, -mu));
+            ps0 += a;
+            ps1 += b;
+            pk[i >> 1] = BF ? pack_bf16x2(a, b) : pack_half2(a, b);
+          }
+          tmem_st16(tS + c * 16, pk);
+        };
+        if (p.bf16) {
+          to_p(std::true_type{}, s0, 0);
+          to_p(std::true_type{}, s1, 1);
+          to_p(std::true_type{}, s2, 2);
+          to_p(std::true_type{}, s3, 3);
+        } else {
+          to_p(std::false_type{}, s0, 0);
+          to_p(std::false_type{}, s1, 1);
+          to_p(std::false_type{}, s2, 2);
+          to_p(std::false_type{}, s3, 3);
+        }
+        l += ps0 + ps1;
+        if (kb + kPmBK > it.nk && (t == 0 || j >= na)) {
+          // rows of V past the sequence's end are cleared by the tile whose product comes first
+          const uint32_t iv = ring + 2 * j + 1;
+          if (!__all_sync(0xffffffffu, mbar_wait(&full[iv % kPmSlots], (iv / kPmSlots) & 1))) { timed_out = true; break; }
+          uint8_t* v = sKV + (iv % kPmSlots) * kPmTile;
+          const int r0 = it.nk - kb;
+          for (int e = row; e < (kPmBK - r0) * 16; e += 128) {
+            const int r = r0 + (e >> 4), c = e & 15;
+            *reinterpret_cast<uint4*>(v + (c >> 3) * kPmHalf + swz128(r, c & 7)) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async();
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+      }
+      if (timed_out) break;
+      ring += 2 * nblk;
+
+      // ---- the row's result
+      if (mine > 0) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&o_full[t], n_o++ & 1))) { timed_out = true; break; }
+        tc_fence_after();
+      }
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;           // 0: the row saw no key (a NaN stays one)
+      __half* dst = p.out + ((size_t)(it.tok0 + tk) * p.Hq + (size_t)h * p.G + g) * kPmD;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        if (mine > 0) {
+          tmem_ld32(tO + c * 32, o);
+          tmem_ld_wait();
+        }
+        if (!valid) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint4 w = make_uint4(0u, 0u, 0u, 0u);
+          if (mine > 0 && inv != 0.f) {
+            w.x = pack2(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv, p.bf16);
+            w.y = pack2(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv, p.bf16);
+            w.z = pack2(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv, p.bf16);
+            w.w = pack2(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv, p.bf16);
+          }
+          reinterpret_cast<uint4*>(dst + c * 32)[i] = w;
+        }
+      }
+      tc_fence_before();                                  // these loads before the p_full of the next unit
+    }
+  }
+  if (timed_out) report(p.status, kStatusTimeout);
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_free(tmem_base, kPmCols);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------
+static int prompt_tiles_bound(int Tq, int S, int tpt) {
+  const long long n = (long long)Tq / (2 * tpt) + S;       // each sequence ends with at most one partial tile
+  return n > 0x7fffffffll / 64 ? -1 : (int)n;
+}
+
+static size_t prompt_ws(int n) { return 256 + (size_t)n * sizeof(PromptItem); }
+
+struct PromptStrides {
+  long long tok, head;       // elements
+};
+
+static int prompt_impl(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
+                       const int32_t* lens, const int32_t* page_table, int pages, int page_size, int table_stride,
+                       PromptStrides sq, PromptStrides sk, PromptStrides sv, void* out, int S, int Tq, int Tk, int Hq, int Hkv,
+                       int D, int causal, int bf16, void* ws, size_t ws_bytes, int32_t* status, cudaStream_t stream) {
+  auto bad_ptr = [](const void* x, uintptr_t a) { return x == nullptr || (reinterpret_cast<uintptr_t>(x) & (a - 1)) != 0; };
+  const bool paged = lens != nullptr;
+  if (S < 0 || Tq < 0 || Tk < 0 || Hq <= 0 || Hkv <= 0 || (bf16 != 0 && bf16 != 1) || (causal != 0 && causal != 1)) return VMK_E_BADARG;
+  if (D != kPmD || Hq % Hkv != 0 || Hq / Hkv > 16) return VMK_E_UNSUPPORTED;
+  if (Tq == 0) return VMK_OK;
+  if (bad_ptr(q, 16) || bad_ptr(out, 16) || bad_ptr(cu_q, 4) || (status && bad_ptr(status, 4))) return VMK_E_BADARG;
+  const bool keys = paged ? pages > 0 : Tk > 0;
+  if (keys && (bad_ptr(k, 16) || bad_ptr(v, 16))) return VMK_E_BADARG;
+  if (paged) {
+    if (bad_ptr(page_table, 4) || bad_ptr(lens, 4) || pages < 0 || page_size <= 0 || page_size % 64 != 0 || table_stride <= 0) return VMK_E_BADARG;
+    if ((long long)pages * Hkv > 0x7fffffffll) return VMK_E_TOO_LARGE;
+  } else if (bad_ptr(cu_k, 4)) {
+    return VMK_E_BADARG;
+  }
+  if (Tk > 0x7fff0000 || Tq > 0x7fff0000) return VMK_E_TOO_LARGE;
+  const int G = Hq / Hkv, tpt = 128 / G;
+  const int max_items = prompt_tiles_bound(Tq, S, tpt);
+  if (max_items < 0 || (long long)max_items * Hkv > 0x3fffffffll) return VMK_E_TOO_LARGE;
+  if (bad_ptr(ws, 256)) return VMK_E_BADARG;
+  if (ws_bytes < prompt_ws(max_items)) return VMK_E_WORKSPACE;
+
+  PromptParams p;
+  memset(&p, 0, sizeof(p));
+  int rc = make_tmap_strided(&p.tmQ, q, (uint64_t)Hq, (uint64_t)Tq, sq.head, sq.tok, 64, G, tpt);
+  if (rc != VMK_OK) return rc;
+  if (keys) {
+    if (paged) {
+      rc = make_tmap_3d(&p.tmK, k, kPmD, page_size, (uint64_t)pages * Hkv, 64, 64);
+      if (rc == VMK_OK) rc = make_tmap_3d(&p.tmV, v, kPmD, page_size, (uint64_t)pages * Hkv, 64, 64);
+    } else {
+      rc = make_tmap_strided(&p.tmK, k, (uint64_t)Hkv, (uint64_t)Tk, sk.head, sk.tok, 64, 1, kPmBK);
+      if (rc == VMK_OK) rc = make_tmap_strided(&p.tmV, v, (uint64_t)Hkv, (uint64_t)Tk, sv.head, sv.tok, 64, 1, kPmBK);
+    }
+    if (rc != VMK_OK) return rc;
+  } else {
+    p.tmK = p.tmV = p.tmQ;                                 // valid descriptors that no load uses
+  }
+  static std::atomic<uint64_t> configured{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return VMK_E_LAUNCH;
+  if (dev >= 64 || !(configured.load() >> dev & 1)) {
+    const cudaError_t e = cudaFuncSetAttribute(prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPmSmem);
+    if (e != cudaSuccess) return check_launch(e);
+    if (dev < 64) configured.fetch_or(1ull << dev);
+  }
+  p.out = static_cast<__half*>(out);
+  p.ctrl = static_cast<PromptCtrl*>(ws);
+  PromptItem* items = reinterpret_cast<PromptItem*>(static_cast<uint8_t*>(ws) + 256);
+  p.items = items;
+  p.page_table = paged ? page_table : nullptr;
+  p.page_size = page_size;
+  p.table_stride = table_stride;
+  p.page_groups = paged ? pages * Hkv : 0;
+  p.Tq = Tq;
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  p.G = G;
+  p.tpt = tpt;
+  p.sc = kLog2e * 0.08838834764831845f;                    // log2(e) / sqrt(128)
+  p.bf16 = bf16;
+  p.status = status;
+  const long long units = (long long)max_items * Hkv;
+  const int grid = (int)(units < 1 ? 1 : units < sm_count() ? units : sm_count());
+
+  PromptPlanParams pp;
+  memset(&pp, 0, sizeof(pp));
+  pp.cu_q = cu_q;
+  pp.cu_k = cu_k;
+  pp.lens = lens;
+  pp.items = items;
+  pp.ctrl = p.ctrl;
+  pp.S = S;
+  pp.Tq = Tq;
+  const long long cap = (long long)table_stride * page_size;
+  pp.Tk = !keys ? 0 : paged ? (int)(cap > 0x7fff0000ll ? 0x7fff0000ll : cap) : Tk;
+  pp.tpt = tpt;
+  pp.causal = causal;
+  pp.max_items = max_items;
+  pp.first_units = grid;
+  pp.status = status;
+
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(1);
+  cfg.blockDim = dim3(kPmPlanThreads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  rc = check_launch(cudaLaunchKernelEx(&cfg, prompt_plan_kernel, pp));
+  if (rc != VMK_OK) return rc;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kPmThreads);
+  cfg.dynamicSmemBytes = kPmSmem;
+  return check_launch(cudaLaunchKernelEx(&cfg, prompt_kernel, p));
+}
+
+}  // namespace vmk
+
+using namespace vmk;
+
+extern "C" size_t vmk_prompt_workspace_bytes(int S, int Tq, int Hq, int Hkv, int D) {
+  if (S < 0 || Tq < 0 || Hq <= 0 || Hkv <= 0 || D != kPmD || Hq % Hkv != 0 || Hq / Hkv > 16) return 0;
+  const int n = prompt_tiles_bound(Tq, S, 128 / (Hq / Hkv));
+  return n < 0 ? 0 : prompt_ws(n);
+}
+
+extern "C" int vmk_prompt(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
+                          const int64_t* strides, void* out, int S, int Tq, int Tk, int Hq, int Hkv, int D, int causal,
+                          int bf16, void* ws, size_t ws_bytes, int32_t* status, void* stream) {
+  const long long dq = (long long)Hq * D, dk = (long long)Hkv * D;
+  PromptStrides sq{dq, D}, sk{dk, D}, sv{dk, D};
+  if (strides != nullptr) {
+    sq = {strides[0], strides[1]};
+    sk = {strides[2], strides[3]};
+    sv = {strides[4], strides[5]};
+  }
+  return prompt_impl(q, k, v, cu_q, cu_k, nullptr, nullptr, 0, 0, 0, sq, sk, sv, out, S, Tq, Tk, Hq, Hkv, D, causal, bf16, ws,
+                     ws_bytes, status, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int vmk_prompt_paged(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table, int pages,
+                                int page_size, int table_stride, const int32_t* cu_q, const int32_t* lens,
+                                const int64_t* strides, void* out, int S, int Tq, int Hq, int Hkv, int D, int causal,
+                                int bf16, void* ws, size_t ws_bytes, int32_t* status, void* stream) {
+  if (lens == nullptr) return VMK_E_BADARG;
+  PromptStrides sq{(long long)Hq * D, D};
+  if (strides != nullptr) sq = {strides[0], strides[1]};
+  return prompt_impl(q, k_pages, v_pages, cu_q, nullptr, lens, page_table, pages, page_size, table_stride, sq, sq, sq, out, S,
+                     Tq, 0, Hq, Hkv, D, causal, bf16, ws, ws_bytes, status, static_cast<cudaStream_t>(stream));
+}
