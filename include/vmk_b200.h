@@ -285,6 +285,69 @@ VMK_API int vmk_prompt_paged(const void* q, const void* k_pages, const void* v_p
                              const int64_t* strides, void* out, int S, int Tq, int Hq, int Hkv, int D, int causal,
                              int bf16, void* ws, size_t ws_bytes, int32_t* status, void* stream);
 
+/* ---- accept: which drafts of a speculative tree stand ----------------------------------------------------
+ * The step after vmk_spec_verify, once every draft row has its probabilities; the reference stops at the attention
+ * (kernels/spec_opus55_v7.py:467-521).  Node 0 of a request's tree is decided already; the parent of node i is the
+ * highest node below i in row i of bits (layout of vmk_spec_verify: bits_words words a row, kd <= 32 * bits_words,
+ * kd <= VMK_SPEC_MAX_DRAFTS).
+ *   target_probs, draft_probs (B,kd,V): dtype 0 fp32, 1 fp16, 2 bf16, aligned to their elements.  Row c: the target's distribution after node c, and
+ *   the one that the children of c were drawn from, each by itself; draft_probs null: drafts that were chosen, not drawn.
+ *   tokens (B,kd) int32;  u (B,kd) fp32 in [0,1): u[i] decides on node i, u[0] draws the next token.
+ *   path (B,kd) int32: the accepted nodes, path[0] = 0, -1 behind them;  count (B): how many;  next (B): the token after
+ *   the last of them, -1 where its row of target_probs holds nothing positive.
+ * At a node with S = 0, M = 1: child i with token x is accepted iff u[i] M q(x) < r(x) with r = max(p - S q, 0); if not,
+ * S += M and M = sum(r) with the new S.  Without draft_probs: accepted iff u[i] M < r(x) with r = p without the tokens
+ * refused so far; if not, M -= r(x).  next is the first entry whose cumulative sum of r (of p where r is empty) exceeds
+ * u[0] times the whole sum.  All in 64 bits; NaN, infinite and negative entries count as 0; a token outside [0, V) is
+ * refused (status). */
+VMK_API int vmk_accept(const void* target_probs, const void* draft_probs, const int32_t* tokens, const uint32_t* bits,
+                       int bits_words, const float* u, int32_t* path, int32_t* count, int32_t* next, int B, int kd, int V,
+                       int dtype, int32_t* status, void* stream);
+
+/* ---- pages: the pages of a paged cache ---------------------------------------------------------------------
+ * What keeps the tables that the *_paged entry points read (the reference names the paged cache as left out,
+ * README.md:141-142).  State, all int32 on the device: page_table (R, table_stride), slot i of row r = the page of its
+ * positions [i * page_size, (i+1) * page_size), -1 behind them; lens (R); refs (pages), 16-byte aligned: the number of
+ * slots that name a page.  A page with refs 0 is free.  Pages are given lowest first, to rows (entries) in their order; one
+ * gets all that it asks for or, where the pages needed by it and all before it exceed the free ones, none (status bit 2).
+ * table_stride <= 2^20.  Calls on the same state belong on one stream.
+ *   pools: HOST array of four int64 per pool: device address (16-byte aligned), layers, heads, bytes of one position of
+ *   one head (a multiple of 16): a contiguous tensor (layers, pages, heads, page_size, bytes).  Up to 8 pools.
+ * vmk_pages_reserve: row r grows by extra[r] >= 0 positions: gets the pages, lens[r] += extra[r].  granted (R), nullable: 1
+ *   or 0.  A row whose table would be too short is refused (status bit 2).
+ * vmk_pages_append: writes tokens into two pools of one layer each (keys and values): sources = HOST array of three
+ *   int64 for each: address, token stride and head stride in bytes (multiples of 16).  Token t of the packed tokens
+ *   [cu[s], cu[s+1]) of row s goes to position lens[s] - (cu[s+1] - t): lens counts the new tokens already.  Tokens
+ *   outside [cu[0], cu[S]) are not written; nor are those without a page (status bit 1).
+ * vmk_pages_fork: entry f makes row children[f] (of length 0) a copy of row parents[f]: full pages are shared (refs + 1), of
+ *   a last page that is not full a new page gets the used rows, in every pool.  parents[f] < 0: nothing to do.  A child
+ *   that is not empty, is named twice (the first has it) or out of range is refused (status bit 1).
+ * vmk_pages_compact: after a verification of kd drafts at the end of each row: the accepted ones, path[r][0 .. count[r])
+ *   ascending (as vmk_accept gives them), close up behind the rest, lens[r] becomes lens[r] - kd + count[r], and pages
+ *   behind that are given back.  count[r] < 0: the row stays as it is.  Drafts in a page that other rows share are not
+ *   moved (status bit 2); a path that does not ascend is not followed where it does not (status bit 1).  kd <= 128.
+ * vmk_pages_free: row r keeps its first keep[r] >= 0 positions and gives back (refs - 1) the pages behind them; its freed
+ *   slots become -1.
+ * vmk_pages_copy: page src[i] -> page dst[i] in every pool, i < n; a page is not both among src and dst, nor twice in dst.
+ * Workspace of reserve (R, 0, pages) and fork (R, F, 0), 16-byte aligned: vmk_pages_workspace_bytes. */
+VMK_API size_t vmk_pages_workspace_bytes(int R, int F, int pages);
+VMK_API int vmk_pages_reserve(int32_t* page_table, int R, int table_stride, int32_t* lens, int32_t* refs, int pages,
+                              int page_size, const int32_t* extra, int32_t* granted, void* ws, size_t ws_bytes,
+                              int32_t* status, void* stream);
+VMK_API int vmk_pages_append(const int64_t* pools, const int64_t* sources, int pages, int page_size,
+                             const int32_t* page_table, int table_stride, const int32_t* cu, const int32_t* lens, int S,
+                             int tokens, int32_t* status, void* stream);
+VMK_API int vmk_pages_fork(const int64_t* pools, int n_pools, int32_t* page_table, int R, int table_stride, int32_t* lens,
+                           int32_t* refs, int pages, int page_size, const int32_t* parents, const int32_t* children, int F,
+                           void* ws, size_t ws_bytes, int32_t* status, void* stream);
+VMK_API int vmk_pages_compact(const int64_t* pools, int n_pools, int32_t* page_table, int R, int table_stride, int32_t* lens,
+                              int32_t* refs, int pages, int page_size, const int32_t* path, const int32_t* count, int kd,
+                              int32_t* status, void* stream);
+VMK_API int vmk_pages_free(int32_t* page_table, int R, int table_stride, int32_t* lens, int32_t* refs, int pages,
+                           int page_size, const int32_t* keep, int32_t* status, void* stream);
+VMK_API int vmk_pages_copy(const int64_t* pools, int n_pools, int pages, int page_size, const int32_t* src,
+                           const int32_t* dst, int n, int32_t* status, void* stream);
+
 /* ---- merge of split partials -------------------------------------------------------------------
  * Log-sum-exp merge used after a KV split across GPUs (the reference merges its in-GPU splits the
  * same way, kernels/prefix_opus55_v8.py:211-261).  m, l (parts,rows) and o (parts,rows,D) fp32 with m

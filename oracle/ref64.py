@@ -189,3 +189,55 @@ def prompt_ref64(q, k, v, nq, nk, causal=True):
                     s[tq + i, h] = (np.abs(kk[:c]) @ np.abs(q[tq + i, h])).max() / math.sqrt(D)
         tq, tk = tq + n, tk + m
     return out, a, s
+
+
+def accept_ref64(target_probs, tokens, bits, u, draft_probs=None, **_):
+    """Acceptance of drafts (no counterpart in the reference, which verifies their attention, ops/spec.py:69-82): the
+    residual kept as a vector, normalised again after every refusal.  Returns (path, count, next) as the op does, and
+    per request how near its closest decision was: |difference| of the two sides of each comparison over their size
+    (a decision within rounding of its border says nothing)."""
+    def clean(x):
+        x = np.asarray(x).astype(np.float64)
+        return np.where(np.isfinite(x) & (x > 0), x, 0.0)
+    B, kd, V = np.asarray(target_probs).shape
+    words = np.asarray(bits).reshape(B, kd, -1).astype(np.int64) & 0xFFFFFFFF
+    path = np.full((B, kd), -1, dtype=np.int32)
+    count, nxt, near = np.zeros(B, np.int32), np.full(B, -1, np.int32), np.full(B, np.inf)
+    for b in range(B):
+        masks = [sum(int(w) << (32 * j) for j, w in enumerate(words[b, i])) for i in range(kd)]
+        parent = [(masks[i] & ((1 << i) - 1)).bit_length() - 1 for i in range(kd)]
+        cur, n = 0, 1
+        path[b, 0] = 0
+        while True:
+            p = clean(target_probs[b, cur])
+            q = None if draft_probs is None else clean(draft_probs[b, cur])
+            r, mass, step = p.copy(), 1.0, None
+            for i in (i for i in range(1, kd) if parent[i] == cur):
+                x = int(tokens[b, i])
+                rx, qx = (r[x], 1.0 if q is None else q[x]) if 0 <= x < V else (0.0, 0.0)
+                bar = float(u[b, i]) * mass * qx
+                if rx > 0:
+                    near[b] = min(near[b], abs(bar - rx) / max(bar, rx))
+                if rx > 0 and bar < rx:
+                    step = i
+                    break
+                if q is None:
+                    mass = max(mass - rx, 0.0)
+                    if 0 <= x < V:
+                        r[x] = 0.0
+                else:
+                    r = np.maximum(r - mass * q, 0.0)
+                    mass = float(r.sum())
+            if step is None:
+                break
+            cur = step
+            path[b, n] = step
+            n += 1
+        count[b] = n
+        w = r if r.sum() > 0 else p
+        c = np.cumsum(w)
+        if c[-1] > 0:
+            hit = np.nonzero((c > float(u[b, 0]) * c[-1]) & (w > 0))[0]
+            nxt[b] = hit[0] if hit.size else np.nonzero(w > 0)[0][-1]
+            near[b] = min(near[b], float(np.abs(c / c[-1] - float(u[b, 0])).min()))
+    return path, count, nxt, near

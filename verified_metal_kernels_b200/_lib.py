@@ -46,6 +46,14 @@ SIGNATURES = {
     "vmk_prompt_workspace_bytes": (_sz, [_i] * 5),
     "vmk_prompt": (_i, [_vp] * 7 + [_i] * 8 + [_vp, _sz, _vp, _vp]),
     "vmk_prompt_paged": (_i, [_vp] * 4 + [_i] * 3 + [_vp] * 4 + [_i] * 7 + [_vp, _sz, _vp, _vp]),
+    "vmk_accept": (_i, [_vp] * 4 + [_i] + [_vp] * 4 + [_i] * 4 + [_vp, _vp]),
+    "vmk_pages_workspace_bytes": (_sz, [_i] * 3),
+    "vmk_pages_reserve": (_i, [_vp, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _sz, _vp, _vp]),
+    "vmk_pages_append": (_i, [_vp, _vp, _i, _i, _vp, _i, _vp, _vp, _i, _i, _vp, _vp]),
+    "vmk_pages_fork": (_i, [_vp, _i, _vp, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _sz, _vp, _vp]),
+    "vmk_pages_compact": (_i, [_vp, _i, _vp, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _vp]),
+    "vmk_pages_free": (_i, [_vp, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _vp]),
+    "vmk_pages_copy": (_i, [_vp, _i, _i, _i, _vp, _vp, _i, _vp, _vp]),
     "vmk_lse_merge": (_i, [_vp] * 3 + [_i] * 3 + [_vp, _vp]),
     "vmk_prefix_partial": (_i, [_vp] * 6 + [_i] * 9 + [_vp] * 3 + [_vp, _sz, _vp, _vp]),
     "vmk_spec_partial": (_i, [_vp] * 4 + [_i] + [_i] * 8 + [_vp] * 3 + [_vp, _sz, _vp, _vp]),

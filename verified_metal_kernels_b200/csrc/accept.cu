@@ -1,0 +1,418 @@
+// Which drafts of a speculative tree stand: the step after `spec`, which gives every draft row its logits.  The reference
+// verifies attention only (kernels/spec_opus55_v7.py:467-521); the float64 statement lives in oracle/ref64.py (accept_ref64).
+//
+// Node 0 of a request's tree is the token that is decided already, row c of target_probs is the target's distribution
+// after node c, row c of draft_probs the one that c's children were drawn from.  At a node, its children are tried in
+// their order; with r_0 = p, a child with token x stands with probability min(1, r(x) / q(x)), and after a refusal the
+// target is what the draft left of it, r_{j+1} = max(r_j - q, 0) normalised again.  Kept without normalising:
+//     r_j = max(r_{j-1} - M_{j-1} q, 0),  M_j = sum r_j,  M_0 = 1       (M: what the normalised one is divided by)
+//         = max(p - S_j q, 0)  with  S_j = M_0 + ... + M_{j-1}          (once an entry is 0 it stays 0)
+// so a node's state is two numbers, and a refusal is one pass over a row of p and of q.  A child is taken when
+// u M q(x) < r(x).  Without draft_probs the drafts were chosen, not drawn (q = 1 at x): a refusal takes x out of r and
+// r(x) off M, which needs no pass.  When no child is left the next token is drawn from r (from p at a leaf, or if r is
+// empty) by the inverse of its cumulative sum at the root's number.
+//
+// Everything is computed in 64 bits: the answers are whole numbers, and an fp32 sum over a vocabulary is off by more
+// than the width of a rare token.  Products and differences are rounded one by one (no fused multiply-add), so a plain
+// 64-bit evaluation gives the same bits but for the order of the sums.  Entries that are NaN, infinite or negative
+// count as 0.
+//
+// Of a request's kd rows only those are read at which a draft is refused or the walk ends; the rest of the walk needs
+// p and q at (parent, token) of each node, gathered by one thread a node before it begins.  A request is a CLUSTER of
+// up to 8 CTAs that walk its tree in step and split the vocabulary between them: partial sums cross through distributed
+// shared memory.  Inside a CTA every warp owns a contiguous range of the row, so the drawn position is found by prefix
+// over CTAs, then warps, then one warp's range.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+
+#include <cstring>
+
+#include "common.cuh"
+
+namespace vmk {
+
+namespace cg = cooperative_groups;
+
+constexpr int kAcThreads = 512;
+constexpr int kAcWarps = kAcThreads / 32;
+constexpr int kAcNodes = VMK_SPEC_MAX_DRAFTS;
+constexpr int kAcCluster = 8;
+
+struct AcceptParams {
+  const void *p, *q;             // (B, kd, V), q null: drafts without probabilities
+  const int32_t* tokens;         // (B, kd)
+  const uint32_t* bits;          // (B, kd, words)
+  const float* u;                // (B, kd)
+  int32_t *path, *count, *next;  // (B, kd), (B), (B)
+  int kd, words, V;
+  int32_t* status;
+};
+
+struct AcceptShared {
+  double p[kAcNodes], q[kAcNodes], u[kAcNodes];
+  int token[kAcNodes], parent[kAcNodes];
+  int gone[kAcNodes];            // tokens refused at the current node (drafts without probabilities)
+  int path[kAcNodes];
+  double warp_sum[kAcWarps];
+  double rank_sum[2][kAcCluster];   // every CTA's sum of a pass; alternating, so that one barrier a pass is enough
+};
+
+// Sanitised probability: positive and finite, else 0.
+__device__ __forceinline__ float ac_clean(float x) {
+  return __float_as_uint(x) - 1u < 0x7f7fffffu ? x : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ float ac_float(T x);
+template <>
+__device__ __forceinline__ float ac_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float ac_float<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float ac_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+template <typename T>
+struct AcVec {
+  static constexpr int N = 16 / sizeof(T);
+  union {
+    uint4 raw;
+    T e[N];
+  };
+  __device__ AcVec() {}
+};
+
+// A row of V probabilities as 16-byte vectors: rows of an odd length begin inside one.  Vector i holds the elements
+// [i * N - head, (i + 1) * N - head); those outside the row are 0.
+template <typename T>
+__device__ __forceinline__ void ac_load(AcVec<T>& v, const T* row, int head, int V, int i, bool aligned = true) {
+  constexpr int N = AcVec<T>::N;
+  const int e0 = i * N - head;
+  if (aligned && e0 >= 0 && e0 + N <= V) {
+    v.raw = __ldg(reinterpret_cast<const uint4*>(row + e0));
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) v.e[k] = (e0 + k >= 0 && e0 + k < V) ? row[e0 + k] : T(0.f);
+  }
+}
+
+// Weights of one vector: max(p - S q, 0), or p without the refused tokens.
+template <typename T, bool HAS_Q>
+__device__ __forceinline__ void ac_weights(double (&w)[AcVec<T>::N], const AcVec<T>& p, const AcVec<T>& q, double S, bool minus_q,
+                                           const int* gone, int n_gone, int e0) {
+  constexpr int N = AcVec<T>::N;
+#pragma unroll
+  for (int k = 0; k < N; ++k) w[k] = (double)ac_clean(ac_float<T>(p.e[k]));
+  if (HAS_Q) {
+    if (minus_q) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const double d = __dsub_rn(w[k], __dmul_rn(S, (double)ac_clean(ac_float<T>(q.e[k]))));
+        w[k] = d > 0.0 ? d : 0.0;
+      }
+    }
+  } else {
+    for (int g = 0; g < n_gone; ++g) {
+      const int k0 = gone[g] - e0;
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (k == k0) w[k] = 0.0;
+    }
+  }
+}
+
+template <typename T, bool HAS_Q>
+__global__ void __launch_bounds__(kAcThreads) accept_kernel(const AcceptParams a) {
+  constexpr int N = AcVec<T>::N;
+  __shared__ AcceptShared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
+  const int b = blockIdx.x / ranks;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int kd = a.kd, V = a.V;
+  pdl_wait();
+
+  // ---- the tree, and the two probabilities of every node
+  const size_t node0 = (size_t)b * kd;
+  if (tid < kd) {
+    const uint32_t* words = a.bits + (node0 + tid) * a.words;
+    int parent = -1;
+    for (int w = (tid - 1) >> 5; w >= 0 && parent < 0 && tid > 0; --w) {
+      uint32_t m = w < a.words ? words[w] : 0u;
+      if (w == tid >> 5) m &= (1u << (tid & 31)) - 1u;
+      if (m != 0u) parent = w * 32 + 31 - __clz(m);
+    }
+    const int x = a.tokens[node0 + tid];
+    const bool inside = x >= 0 && x < V;
+    float p = 0.f, q = 0.f;
+    if (tid > 0 && parent >= 0 && inside) {
+      const size_t at = (node0 + parent) * V + x;
+      p = ac_clean(ac_float<T>(static_cast<const T*>(a.p)[at]));
+      if (HAS_Q) q = ac_clean(ac_float<T>(static_cast<const T*>(a.q)[at]));
+    }
+    if (tid > 0 && !inside && rank == 0) report(a.status, kStatusBadIndex);
+    sh.parent[tid] = parent;
+    sh.token[tid] = x;
+    sh.p[tid] = p;
+    sh.q[tid] = q;
+    sh.u[tid] = a.u[node0 + tid];
+    sh.path[tid] = tid == 0 ? 0 : -1;
+  }
+  cluster.sync();                                // and every peer runs before anything is written into its shared memory
+
+  int mine[kAcNodes / 32];                       // every warp: parents of the nodes lane, lane + 32, ...
+#pragma unroll
+  for (int w = 0; w < kAcNodes / 32; ++w) mine[w] = w * 32 + lane < kd ? sh.parent[w * 32 + lane] : -1;
+
+  int cur = 0, n_path = 1, n_gone = 0, passes = 0;
+  double S = 0.0, M = 1.0;
+  int head = 0, nvec = 0, seg = 0, seg0 = 0;     // this warp's vectors of the row: [seg0, min(seg0 + seg, nvec))
+  const T *prow = nullptr, *qrow = nullptr;
+  bool q16 = true;                               // rows of p and q begin at the same place of a 16-byte vector
+
+  // Sum of the current weights over the row: every CTA's in rank_sum, every warp's of this CTA in warp_sum.
+  auto pass = [&](bool minus_q) -> double {
+    prow = static_cast<const T*>(a.p) + (node0 + cur) * V;
+    qrow = HAS_Q ? static_cast<const T*>(a.q) + (node0 + cur) * V : prow;
+    q16 = ((reinterpret_cast<uintptr_t>(prow) ^ reinterpret_cast<uintptr_t>(qrow)) & 15) == 0;
+    head = (int)((reinterpret_cast<uintptr_t>(prow) & 15) / sizeof(T));
+    nvec = (head + V + N - 1) / N;
+    seg = (nvec + ranks * kAcWarps - 1) / (ranks * kAcWarps);
+    seg0 = (rank * kAcWarps + warp) * seg;
+    const int end = min(seg0 + seg, nvec);
+    double sum[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int i = seg0 + lane; i < end; i += 4 * 32) {
+      AcVec<T> p[4], q[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (i + k * 32 < end) {
+          ac_load<T>(p[k], prow, head, V, i + k * 32);
+          if (HAS_Q && minus_q) ac_load<T>(q[k], qrow, head, V, i + k * 32, q16);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (i + k * 32 < end) {
+          double w[N];
+          ac_weights<T, HAS_Q>(w, p[k], q[k], S, minus_q, sh.gone, n_gone, (i + k * 32) * N - head);
+#pragma unroll
+          for (int e = 0; e < N; ++e) sum[e & 3] += w[e];
+        }
+      }
+    }
+    double t = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    __syncthreads();                             // readers of the pass before are done with warp_sum
+    if (lane == 0) sh.warp_sum[warp] = t;
+    __syncthreads();
+    double* mine_sum = &sh.rank_sum[passes & 1][0];
+    if (tid < ranks) {
+      double all = 0.0;
+      for (int w = 0; w < kAcWarps; ++w) all += sh.warp_sum[w];
+      *cluster.map_shared_rank(mine_sum + rank, tid) = all;
+    }
+    cluster.sync();
+    double total = 0.0;
+    for (int r = 0; r < ranks; ++r) total += mine_sum[r];
+    ++passes;
+    return total;
+  };
+
+  // ---- the walk, the same in every thread of the cluster
+  double T_left = 0.0;                           // sum of the weights of the last pass
+  bool have_sum = false;
+  for (;;) {
+    bool moved = false;
+#pragma unroll
+    for (int w = 0; w < kAcNodes / 32; ++w) {
+      uint32_t kids = __ballot_sync(0xffffffffu, !moved && mine[w] == cur);
+      while (kids != 0u && !moved) {
+        const int i = w * 32 + __ffs(kids) - 1;
+        kids &= kids - 1u;
+        const double p = sh.p[i], q = sh.q[i], u = sh.u[i];
+        double r;
+        bool yes;
+        if (HAS_Q) {
+          r = __dsub_rn(p, __dmul_rn(S, q));
+          yes = r > 0.0 && __dmul_rn(__dmul_rn(u, M), q) < r;
+        } else {
+          r = p;
+          const int x = sh.token[i];
+          for (int g = 0; g < n_gone; ++g)
+            if (sh.gone[g] == x) r = 0.0;
+          yes = r > 0.0 && __dmul_rn(u, M) < r;
+        }
+        if (yes) {
+          cur = i;
+          if (tid == 0) sh.path[n_path] = i;
+          ++n_path;
+          S = 0.0;
+          M = 1.0;
+          n_gone = 0;
+          have_sum = false;
+          moved = true;
+        } else if (HAS_Q) {
+          S += M;
+          M = pass(true);
+          T_left = M;
+          have_sum = true;
+        } else {
+          M = fmax(__dsub_rn(M, r), 0.0);
+          __syncthreads();                       // nobody is still reading the list
+          if (tid == 0) sh.gone[n_gone] = sh.token[i];
+          ++n_gone;
+          __syncthreads();
+        }
+      }
+    }
+    if (!moved) break;
+  }
+
+  // ---- the next token
+  bool minus_q = HAS_Q && S > 0.0;
+  if (!have_sum) T_left = pass(minus_q);
+  if (!(T_left > 0.0) && (minus_q || n_gone > 0)) {
+    minus_q = false;                             // the residual is empty: the target itself
+    n_gone = 0;
+    T_left = pass(false);
+  }
+  int token = -1;
+  const double* rank_sum = sh.rank_sum[(passes - 1) & 1];
+  if (T_left > 0.0) {
+    const double target = __dmul_rn(sh.u[0], T_left);
+    // first CTA, then first warp of it, whose running sum exceeds the target; the last one that has anything if none does
+    int owner = -1, last = 0;
+    double before = 0.0, before_last = 0.0, run = 0.0;
+    for (int r = 0; r < ranks; ++r) {
+      const double s = rank_sum[r];
+      if (s > 0.0) { last = r; before_last = run; }
+      if (owner < 0 && s > 0.0 && run + s > target) { owner = r; before = run; }
+      run += s;
+    }
+    if (owner < 0) { owner = last; before = before_last; }
+    if (owner == rank) {
+      int ow = -1, lw = 0;
+      double wb = 0.0, wbl = 0.0;
+      run = before;
+      for (int w = 0; w < kAcWarps; ++w) {
+        const double s = sh.warp_sum[w];
+        if (s > 0.0) { lw = w; wbl = run; }
+        if (ow < 0 && s > 0.0 && run + s > target) { ow = w; wb = run; }
+        run += s;
+      }
+      if (ow < 0) { ow = lw; wb = wbl; }
+      if (ow == warp) {
+        const int end = min(seg0 + seg, nvec);
+        run = wb;
+        int found = -1, positive = -1;
+        for (int i0 = seg0; i0 < end && found < 0; i0 += 32) {
+          const int i = i0 + lane;
+          double w[N];
+#pragma unroll
+          for (int e = 0; e < N; ++e) w[e] = 0.0;
+          if (i < end) {
+            AcVec<T> p, q;
+            ac_load<T>(p, prow, head, V, i);
+            if (HAS_Q && minus_q) ac_load<T>(q, qrow, head, V, i, q16);
+            ac_weights<T, HAS_Q>(w, p, q, S, minus_q, sh.gone, n_gone, i * N - head);
+          }
+          double own = 0.0;
+          int my_last = -1;
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            own += w[e];
+            if (w[e] > 0.0) my_last = i * N - head + e;
+          }
+          double incl = own;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const double x = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += x;
+          }
+          double c = run + (incl - own);
+          int hit = -1;
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            c += w[e];
+            if (hit < 0 && w[e] > 0.0 && c > target) hit = i * N - head + e;
+          }
+          const uint32_t any = __ballot_sync(0xffffffffu, hit >= 0), pos = __ballot_sync(0xffffffffu, my_last >= 0);
+          if (any != 0u) found = __shfl_sync(0xffffffffu, hit, __ffs(any) - 1);
+          if (pos != 0u) positive = __shfl_sync(0xffffffffu, my_last, 31 - __clz(pos));
+          run += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        token = found >= 0 ? found : positive;
+        if (lane == 0) a.next[b] = token;
+      }
+    }
+  } else if (rank == 0 && tid == 0) {
+    a.next[b] = -1;
+  }
+  __syncthreads();
+  if (rank == 0) {
+    if (tid < kd) a.path[node0 + tid] = sh.path[tid];
+    if (tid == 0) a.count[b] = n_path;
+  }
+  cluster.sync();                                // nobody leaves while a peer may still write into its shared memory
+}
+
+// CTAs per request: as many as keep all requests resident at two CTAs an SM, with at least 2048 entries each.
+static int accept_cluster(int B, int V) {
+  if (g_batch_invariant) return V >= 4 * 2048 ? 4 : 1;    // by the row alone: the order of the sums must not follow the batch
+  int c = kAcCluster;
+  while (c > 1 && ((long long)B * c > 2ll * sm_count() || V < c * 2048)) c >>= 1;
+  return c;
+}
+
+template <typename T>
+static int accept_launch(const AcceptParams& a, int B, cudaStream_t stream) {
+  const int c = accept_cluster(B, a.V);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = c;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)B * c);
+  cfg.blockDim = dim3(kAcThreads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return check_launch(a.q != nullptr ? cudaLaunchKernelEx(&cfg, accept_kernel<T, true>, a) : cudaLaunchKernelEx(&cfg, accept_kernel<T, false>, a));
+}
+
+}  // namespace vmk
+
+using namespace vmk;
+
+extern "C" int vmk_accept(const void* target_probs, const void* draft_probs, const int32_t* tokens, const uint32_t* bits,
+                          int bits_words, const float* u, int32_t* path, int32_t* count, int32_t* next, int B, int kd, int V,
+                          int dtype, int32_t* status, void* stream) {
+  auto bad = [](const void* x, uintptr_t al) { return x == nullptr || (reinterpret_cast<uintptr_t>(x) & (al - 1)) != 0; };
+  if (B < 0 || kd <= 0 || V <= 0 || bits_words <= 0 || dtype < 0 || dtype > 2) return VMK_E_BADARG;
+  if (kd > kAcNodes || kd > 32 * bits_words) return VMK_E_UNSUPPORTED;
+  if (V > 0x7fffff00 || B > 0x7fffffff / kAcCluster) return VMK_E_TOO_LARGE;
+  if (B == 0) return VMK_OK;
+  const uintptr_t size = dtype == 0 ? 4 : 2;                // rows of an odd length are not aligned either
+  if (bad(target_probs, size) || (draft_probs && bad(draft_probs, size)) || bad(tokens, 4) || bad(bits, 4) || bad(u, 4) || bad(path, 4) ||
+      bad(count, 4) || bad(next, 4) || (status && bad(status, 4)))
+    return VMK_E_BADARG;
+  AcceptParams a;
+  memset(&a, 0, sizeof(a));
+  a.p = target_probs;
+  a.q = draft_probs;
+  a.tokens = tokens;
+  a.bits = bits;
+  a.words = bits_words;
+  a.u = u;
+  a.path = path;
+  a.count = count;
+  a.next = next;
+  a.kd = kd;
+  a.V = V;
+  a.status = status;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == 0 ? accept_launch<float>(a, B, s) : dtype == 1 ? accept_launch<__half>(a, B, s) : accept_launch<__nv_bfloat16>(a, B, s);
+}

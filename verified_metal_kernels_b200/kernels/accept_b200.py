@@ -1,0 +1,59 @@
+"""Kernel module for the acceptance of drafts on B200: which nodes of a speculative tree stand, and the token after them.
+
+Not one of the reference's ops, which verify the attention of the drafts (reference ops/spec.py:14-25 builds the trees):
+it is the step after `spec`, once the target's probabilities of every draft row are known."""
+import torch
+
+from .. import _lib
+from ._common import need, stage_in
+
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def kernel(target_probs, tokens, bits, u, draft_probs=None, check=False):
+    """target_probs (B,kd,V) fp32, fp16 or bf16, tokens (B,kd) int32, bits (B,kd) int32 -- or (B,kd,W) words for kd > 32 --
+    as `spec` takes them, u (B,kd) float32 in [0, 1), draft_probs like target_probs or None -> (path (B,kd) int32, count
+    (B,) int32, next_token (B,) int32).
+
+    Node 0 is the root: the token that is decided already.  Node i's parent is the highest node below i in bits[i].  Row c
+    of target_probs is the target's distribution after node c, row c of draft_probs the one that the children of c were
+    drawn from, each by itself; draft_probs=None: the drafts were chosen, not drawn (looked up, or the likeliest).  A
+    node's children are tried in ascending order, child i with the number u[:, i]; u[:, 0] draws the next token, from
+    what is left of the target where the walk ends.  The tokens that come out are distributed as the target's own.
+
+    path: the accepted nodes in order (path[:, 0] = 0), -1 behind them; count: how many.  Computed in 64 bits.  Entries
+    that are NaN, infinite or negative count as 0; a row of nothing but those gives next_token -1.  A draft token outside
+    [0, V) is refused (and reported in the device status word).  Host tensors are copied in and the results returned on
+    the host."""
+    (target_probs, tokens, bits, u, draft_probs), host = stage_in([target_probs, tokens, bits, u, draft_probs])
+    if not isinstance(target_probs, torch.Tensor) or target_probs.dtype not in DTYPES:
+        raise TypeError("target_probs: expected a float32, float16 or bfloat16 tensor")
+    dt = target_probs.dtype
+    need(target_probs, "target_probs", dt, dims=3)
+    B, kd, V = target_probs.shape
+    need(tokens, "tokens", torch.int32, shape=(B, kd))
+    if not isinstance(bits, torch.Tensor) or bits.dtype != torch.int32:
+        raise TypeError("bits: expected an int32 tensor")
+    words = 1 if bits.dim() == 2 else bits.shape[2] if bits.dim() == 3 else 0
+    need(bits, "bits", torch.int32, shape=(B, kd) if bits.dim() == 2 else (B, kd, words))
+    need(u, "u", torch.float32, shape=(B, kd))
+    if draft_probs is not None:
+        need(draft_probs, "draft_probs", dt, shape=(B, kd, V))
+    dev = target_probs.device
+    for name, t in (("tokens", tokens), ("bits", bits), ("u", u), ("draft_probs", draft_probs)):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name}: expected a tensor on {dev}, got {t.device}")
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        stream = torch.cuda.current_stream()
+        out = torch.empty(B * (kd + 2), dtype=torch.int32, device=dev)
+        path, count, token = out[:B * kd].view(B, kd), out[B * kd:B * kd + B], out[B * kd + B:]
+        rc = lib.vmk_accept(_lib.ptr(target_probs), _lib.ptr(draft_probs), _lib.ptr(tokens), _lib.ptr(bits), words, _lib.ptr(u),
+                            _lib.ptr(path), _lib.ptr(count), _lib.ptr(token), B, kd, V, DTYPES[dt],
+                            _lib.ptr(_lib.status_word(dev)), stream.cuda_stream)
+    _lib.check(rc, "vmk_accept")
+    if host:
+        path, count, token = path.cpu(), count.cpu(), token.cpu()
+    if host or check:
+        _lib.raise_on_status(dev, "vmk_accept")
+    return path, count, token

@@ -1,0 +1,201 @@
+"""Kernel module for the pages of a paged cache on B200: what keeps the tables that every kernel_paged(...) reads.
+
+The reference names the paged cache as the variant it left out (README.md:141-142).  State, int32 tensors on the device
+that the calls change in place:
+
+    page_table (R,T)   slot i of row r: the page of its positions [i * page_size, (i+1) * page_size), -1 behind them
+    lens (R,)          positions of each row
+    refs (pages,)      how many slots name a page; 0: the page is free
+
+Pages are given lowest first, to rows in their order.  A pool is a contiguous tensor (pages, heads, page_size, width),
+(layers, pages, heads, page_size, width) or, as dsa's, (pages, page_size, width), of any type whose rows are multiples of
+16 bytes.  Calls on one state belong on one stream; they neither allocate on the host nor synchronise (check=True
+does, and raises on what the device refused: no free page left, an index outside its tensor)."""
+import ctypes
+
+import torch
+
+from .. import _lib
+from ._common import need
+
+
+def _state(page_table, lens, refs):
+    need(page_table, "page_table", torch.int32, dims=2)
+    R, T = page_table.shape
+    need(lens, "lens", torch.int32, shape=(R,))
+    dev = page_table.device
+    _on(dev, lens=lens)
+    if refs is not None:
+        need(refs, "refs", torch.int32, dims=1)
+        _on(dev, refs=refs)
+    return R, T, dev
+
+
+def _on(dev, **tensors):
+    for name, t in tensors.items():
+        if t.device != dev:
+            raise ValueError(f"{name}: expected a tensor on {dev}, got {t.device}")
+
+
+def _pools(pools, dev):
+    """The pools' descriptions (four int64 each), their pages and page size."""
+    if isinstance(pools, torch.Tensor) or not 1 <= len(pools) <= 8:
+        raise ValueError("pools: expected a list of 1 to 8 tensors")
+    d, pages, page_size = [], None, None
+    for i, t in enumerate(pools):
+        name = f"pools[{i}]"
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name}: expected a torch tensor, got {type(t).__name__}")
+        need(t, name, t.dtype)
+        if t.dim() not in (3, 4, 5) or t.numel() == 0:
+            raise ValueError(f"{name}: expected (pages,[heads,]page_size,width) or (layers,pages,heads,page_size,width), got {tuple(t.shape)}")
+        _on(dev, **{name: t})
+        layers = t.shape[0] if t.dim() == 5 else 1
+        shape = t.shape[1:] if t.dim() == 5 else t.shape
+        heads = shape[1] if t.dim() > 3 else 1
+        if pages is None:
+            pages, page_size = shape[0], shape[-2]
+        if (shape[0], shape[-2]) != (pages, page_size):
+            raise ValueError(f"{name}: expected {pages} pages of {page_size} positions, got {shape[0]} of {shape[-2]}")
+        if shape[-1] * t.element_size() % 16:
+            raise ValueError(f"{name}: a position's row must be a multiple of 16 bytes")
+        d += [t.data_ptr(), layers, heads, shape[-1] * t.element_size()]
+    return (ctypes.c_int64 * len(d))(*d), pages, page_size
+
+
+def _need_refs(refs, pages):
+    if refs.shape[0] != pages:
+        raise ValueError(f"refs: expected {pages} entries, one a page, got {refs.shape[0]}")
+
+
+def _done(rc, what, check, dev):
+    _lib.check(rc, what)
+    if check:
+        _lib.raise_on_status(dev, what)
+
+
+def reserve(page_table, lens, refs, extra, page_size, check=False):
+    """Row r grows by extra[r] (>= 0) positions: it gets the pages that it lacks, and lens[r] += extra[r].  A row gets all its
+    pages or, where what it and the rows before it need exceeds the free pages (or its table is too short), none, and
+    stays as it is.  Returns granted (R,) int32, 1 or 0."""
+    R, T, dev = _state(page_table, lens, refs)
+    need(extra, "extra", torch.int32, shape=(R,))
+    _on(dev, extra=extra)
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        stream = torch.cuda.current_stream()
+        granted = torch.empty(R, dtype=torch.int32, device=dev)
+        ws = _lib.scratch(lib.vmk_pages_workspace_bytes(R, 0, refs.shape[0]), dev)
+        rc = lib.vmk_pages_reserve(_lib.ptr(page_table), R, T, _lib.ptr(lens), _lib.ptr(refs), refs.shape[0], page_size, _lib.ptr(extra),
+                                   _lib.ptr(granted), _lib.ptr(ws), ws.numel(), _lib.ptr(_lib.status_word(dev)), stream.cuda_stream)
+    _done(rc, "vmk_pages_reserve", check, dev)
+    return granted
+
+
+def append(k, v, k_pages, v_pages, page_table, cu, lens, check=False):
+    """Writes packed tokens into their pages: k, v (tokens,heads,width) -- views are fine, the innermost axis contiguous --
+    and tokens [cu[s], cu[s+1]) of row s become its last positions: lens[s] counts them already (reserve before append).
+    k_pages, v_pages (pages,heads,page_size,width), or (pages,page_size,width) for one head; k and v may differ in
+    heads and width (dsa: latent rows and index keys).  Tokens outside [cu[0], cu[-1]) are not written."""
+    R, T, dev = _state(page_table, lens, None)
+    need(cu, "cu", torch.int32, dims=1)
+    S = cu.shape[0] - 1
+    if S < 0 or S > R:
+        raise ValueError(f"cu: expected 1 to {R + 1} entries, got {cu.shape[0]}")
+    pools, pages, page_size = _pools([k_pages, v_pages], dev)
+    if k_pages.dim() == 5 or v_pages.dim() == 5:
+        raise ValueError("k_pages, v_pages: expected the pools of one layer")
+    src = []
+    for name, t, pool in (("k", k, k_pages), ("v", v, v_pages)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name}: expected a torch tensor, got {type(t).__name__}")
+        _on(dev, **{name: t})
+        heads = pool.shape[1] if pool.dim() == 4 else 1
+        if t.dtype != pool.dtype:
+            raise TypeError(f"{name}: expected dtype {pool.dtype}, got {t.dtype}")
+        if t.dim() != 3 or tuple(t.shape) != (k.shape[0], heads, pool.shape[-1]):
+            raise ValueError(f"{name}: expected shape ({k.shape[0]}, {heads}, {pool.shape[-1]}), got {tuple(t.shape)}")
+        e = t.element_size()
+        if t.numel() and (t.stride(2) != 1 or t.data_ptr() % 16 or any(n > 1 and (s < 0 or s * e % 16) for n, s in zip(t.shape[:2], t.stride()))):
+            raise ValueError(f"{name}: expected a 16-byte aligned tensor, its innermost axis contiguous, its strides multiples of 16 bytes")
+        src += [t.data_ptr(), t.stride(0) * e if t.shape[0] > 1 else 0, t.stride(1) * e if heads > 1 else 0]
+    _on(dev, cu=cu)
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        stream = torch.cuda.current_stream()
+        rc = lib.vmk_pages_append(pools, (ctypes.c_int64 * 6)(*src), pages, page_size, _lib.ptr(page_table), T, _lib.ptr(cu), _lib.ptr(lens), S,
+                                  k.shape[0], _lib.ptr(_lib.status_word(dev)), stream.cuda_stream)
+    _done(rc, "vmk_pages_append", check, dev)
+
+
+def fork(pools, page_table, lens, refs, parents, children, check=False):
+    """Row children[f] (of length 0) becomes a copy of row parents[f], for every entry f of the two (F,) int32 tensors: full
+    pages are shared, the used rows of a last page that is not full are copied into a page of its own, in every pool.
+    parents[f] < 0: an entry that does nothing.  Refused (and reported): a child that is not empty, out of range, or
+    named a second time; entries for which no free page is left."""
+    R, T, dev = _state(page_table, lens, refs)
+    desc, pages, page_size = _pools(pools, dev)
+    _need_refs(refs, pages)
+    need(parents, "parents", torch.int32, dims=1)
+    F = parents.shape[0]
+    need(children, "children", torch.int32, shape=(F,))
+    _on(dev, parents=parents, children=children)
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        stream = torch.cuda.current_stream()
+        ws = _lib.scratch(lib.vmk_pages_workspace_bytes(R, F, 0), dev)
+        rc = lib.vmk_pages_fork(desc, len(pools), _lib.ptr(page_table), R, T, _lib.ptr(lens), _lib.ptr(refs), pages, page_size, _lib.ptr(parents),
+                                _lib.ptr(children), F, _lib.ptr(ws), ws.numel(), _lib.ptr(_lib.status_word(dev)), stream.cuda_stream)
+    _done(rc, "vmk_pages_fork", check, dev)
+
+
+def compact(pools, page_table, lens, refs, path, count, check=False):
+    """After kd drafts at the end of each row were verified: the accepted ones, path (R,kd) int32 and count (R,) int32 as
+    accept_b200.kernel gives them, close up behind the positions before the drafts, lens[r] becomes lens[r] - kd +
+    count[r], and pages behind that are given back.  count[r] < 0: the row stays as it is."""
+    R, T, dev = _state(page_table, lens, refs)
+    desc, pages, page_size = _pools(pools, dev)
+    _need_refs(refs, pages)
+    need(path, "path", torch.int32, dims=2)
+    kd = path.shape[1]
+    need(path, "path", torch.int32, shape=(R, kd))
+    need(count, "count", torch.int32, shape=(R,))
+    _on(dev, path=path, count=count)
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        stream = torch.cuda.current_stream()
+        rc = lib.vmk_pages_compact(desc, len(pools), _lib.ptr(page_table), R, T, _lib.ptr(lens), _lib.ptr(refs), pages, page_size, _lib.ptr(path),
+                                   _lib.ptr(count), kd, _lib.ptr(_lib.status_word(dev)), stream.cuda_stream)
+    _done(rc, "vmk_pages_compact", check, dev)
+
+
+def free(page_table, lens, refs, keep, page_size, check=False):
+    """Row r keeps its first keep[r] (>= 0) positions; the pages behind them are given back (a page that other rows share
+    stays theirs), and their slots become -1.  keep[r] = 0 frees the row, keep[r] >= lens[r] leaves it as it is."""
+    R, T, dev = _state(page_table, lens, refs)
+    need(keep, "keep", torch.int32, shape=(R,))
+    _on(dev, keep=keep)
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        stream = torch.cuda.current_stream()
+        rc = lib.vmk_pages_free(_lib.ptr(page_table), R, T, _lib.ptr(lens), _lib.ptr(refs), refs.shape[0], page_size, _lib.ptr(keep),
+                                _lib.ptr(_lib.status_word(dev)), stream.cuda_stream)
+    _done(rc, "vmk_pages_free", check, dev)
+
+
+def copy(pools, src, dst, check=False):
+    """Page src[i] -> page dst[i] in every pool and layer; src, dst (n,) int32.  No page may be both in src and in dst, or
+    twice in dst."""
+    if isinstance(pools, torch.Tensor) or not pools or not isinstance(pools[0], torch.Tensor):
+        raise ValueError("pools: expected a list of 1 to 8 tensors")
+    dev = pools[0].device
+    desc, pages, page_size = _pools(pools, dev)
+    need(src, "src", torch.int32, dims=1)
+    need(dst, "dst", torch.int32, shape=tuple(src.shape))
+    _on(dev, src=src, dst=dst)
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        stream = torch.cuda.current_stream()
+        rc = lib.vmk_pages_copy(desc, len(pools), pages, page_size, _lib.ptr(src), _lib.ptr(dst), src.shape[0], _lib.ptr(_lib.status_word(dev)),
+                                stream.cuda_stream)
+    _done(rc, "vmk_pages_copy", check, dev)
