@@ -275,8 +275,9 @@ VMK_API int vmk_dsa_index_project(const void* x, const void* wq, const void* ww,
  *   reaches the rows that see it, and may reach rows before it whose last block of 128 keys holds it.
  * vmk_prompt_paged reads the keys of sequence s from the pages of page_table[s] as vmk_decode_paged does: k_pages,
  * v_pages (pages,Hkv,page_size,D), page_size a multiple of 64, lens (S) int32 = nk (the new tokens included);
- * strides holds the two of q.  A page id outside [0, pages) reads as zeros. */
-VMK_API size_t vmk_prompt_workspace_bytes(int S, int Tq, int Hq, int Hkv, int D);
+ * strides holds the two of q.  A page id outside [0, pages) reads as zeros.
+ * vmk_prompt_workspace_bytes: keys = Tk, or table_stride * page_size. */
+VMK_API size_t vmk_prompt_workspace_bytes(int S, int Tq, long long keys, int Hq, int Hkv, int D);
 VMK_API int vmk_prompt(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,
                        const int64_t* strides, void* out, int S, int Tq, int Tk, int Hq, int Hkv, int D, int causal,
                        int bf16, void* ws, size_t ws_bytes, int32_t* status, void* stream);

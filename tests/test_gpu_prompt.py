@@ -263,3 +263,43 @@ def test_page_ids_outside_the_pool_read_as_zeros():
                                    d["cu_q"], torch.tensor([200], dtype=torch.int32, device="cuda"), check=True)
     inp["k"][64:128], inp["v"][64:128] = 0, 0
     _check(out, inp, seqs, torch.float16)
+
+
+@pytest.mark.parametrize("paged", [False, True], ids=["packed", "paged"])
+@pytest.mark.parametrize("seqs", [[(17, 9001)], [(1, 5000), (3, 700), (2, 0), (5, 2048)], [(64, 1500)], [(40, 513)], [(9, 512), (9, 1024)]], ids=str)
+def test_few_rows_over_many_keys_shared_by_several_ctas(seqs, paged):
+    for dtype in (torch.float16, torch.bfloat16):
+        inp = _inputs(seqs, 8, 2, dtype, seed=83)
+        d = _dev(inp, dtype)
+        if paged:
+            nk = [m for _, m in seqs]
+            kp, vp, table = op.to_pages(inp["k"].astype(np.float32), inp["v"].astype(np.float32), nk, 64, seed=4)
+            out = prompt_b200.kernel_paged(d["q"], torch.from_numpy(kp).cuda().to(dtype), torch.from_numpy(vp).cuda().to(dtype), torch.from_numpy(table).cuda(),
+                                           d["cu_q"], torch.tensor(nk, dtype=torch.int32, device="cuda"), check=True)
+        else:
+            out = prompt_b200.kernel(**d, check=True)
+        _check(out, inp, seqs, dtype)
+        if not paged:
+            _check(prompt_b200.kernel(**d, causal=False, check=True), inp, seqs, dtype, causal=False)
+
+
+def test_batch_invariant_mode_does_not_share():
+    lib = _lib.lib()
+    seqs = [(17, 9001)] + [(30, 30)] * 60
+    inp = _inputs(seqs, 8, 2, torch.float16, seed=89)
+    d = _dev(inp, torch.float16)
+    lib.vmk_set_batch_invariant(1)
+    try:
+        whole = prompt_b200.kernel(**d, check=True)
+        alone = prompt_b200.kernel(d["q"][:17], d["k"][:9001], d["v"][:9001], *(torch.tensor([0, n], dtype=torch.int32, device="cuda") for n in (17, 9001)))
+        assert torch.equal(whole[:17], alone)
+    finally:
+        lib.vmk_set_batch_invariant(0)
+
+
+def test_a_nan_key_in_one_share_reaches_every_row():
+    inp = _inputs([(5, 6000)], 4, 2, torch.float16, seed=97)
+    clean = prompt_b200.kernel(**_dev(inp, torch.float16))
+    inp["k"][3000, 0] = np.nan
+    out = prompt_b200.kernel(**_dev(inp, torch.float16), check=True)
+    assert torch.isnan(out[:, :2]).all() and torch.equal(out[:, 2:], clean[:, 2:])

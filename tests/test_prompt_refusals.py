@@ -45,9 +45,11 @@ def test_c_entry_refuses_before_any_launch(lib):
 
 def test_workspace_sizes(lib):
     f = lib.vmk_prompt_workspace_bytes
-    assert f(1, 128, 32, 8, 128) >= 256 and f(0, 0, 32, 8, 128) >= 256
-    assert f(1, 128, 32, 8, 64) == 0 and f(1, 128, 33, 8, 128) == 0 and f(1, 128, 34, 2, 128) == 0 and f(-1, 1, 8, 8, 128) == 0
-    assert f(1, 1 << 17, 32, 8, 128) < 1 << 20
+    assert f(1, 128, 128, 32, 8, 128) >= 256 and f(0, 0, 0, 32, 8, 128) >= 256
+    assert f(1, 128, 128, 32, 8, 64) == 0 and f(1, 128, 128, 33, 8, 128) == 0 and f(1, 128, 128, 34, 2, 128) == 0
+    assert f(-1, 1, 1, 8, 8, 128) == 0 and f(1, 1, -1, 8, 8, 128) == 0
+    assert f(1, 1 << 17, 1 << 17, 32, 8, 128) < 1 << 20
+    assert 1 << 20 < f(1, 17, 1 << 20, 32, 8, 128) < 1 << 25             # few rows over many keys: the shares' partials
 
 
 def test_module_refuses_by_its_checks(monkeypatch):

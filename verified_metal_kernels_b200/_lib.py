@@ -43,7 +43,7 @@ SIGNATURES = {
     "vmk_dsa_attend_bf16": (_i, [_vp] * 5 + [_i] * 2 + [_vp, _sz, _vp, _vp]),
     "vmk_dsa_gather": (_i, [_vp] * 5 + [_i] * 2 + [_vp, _vp]),
     "vmk_dsa_index_project": (_i, [_vp] * 3 + [_c.c_float] + [_vp] * 2 + [_i] * 3 + [_vp, _vp]),
-    "vmk_prompt_workspace_bytes": (_sz, [_i] * 5),
+    "vmk_prompt_workspace_bytes": (_sz, [_i, _i, _c.c_longlong, _i, _i, _i]),
     "vmk_prompt": (_i, [_vp] * 7 + [_i] * 8 + [_vp, _sz, _vp, _vp]),
     "vmk_prompt_paged": (_i, [_vp] * 4 + [_i] * 3 + [_vp] * 4 + [_i] * 7 + [_vp, _sz, _vp, _vp]),
     "vmk_accept": (_i, [_vp] * 4 + [_i] + [_vp] * 4 + [_i] * 4 + [_vp, _vp]),
@@ -140,11 +140,38 @@ _workspace = Workspace()
 _status = {}
 
 
-def scratch(nbytes, device):
-    """Scratch of one call, from torch's allocator on the current stream: a captured graph keeps its own, and a call
-    on another stream has another."""
+class _Here:
+    """What on_device returns where the device is the current one already."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_here = _Here()
+
+
+def on_device(device):
+    """`with torch.cuda.device(device)`, at no cost where it is the current one."""
     import torch
-    return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def raw_stream(device):
+    """Handle of torch's current stream on `device` (an integer; no Stream object is built)."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def scratch(nbytes, device, stream_id):
+    """Scratch of a call that is made while `device` is the current one.  Under stream capture it is the graph's own (from
+    the graph's memory pool), so that captured graphs do not share it, nor lose it when a larger one takes its place."""
+    import torch
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+    return _workspace.get(nbytes, device, stream_id)
 
 
 def workspace(nbytes, device, stream_id):

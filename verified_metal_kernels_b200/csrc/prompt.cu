@@ -53,6 +53,8 @@ constexpr int kPmCols = 512;
 constexpr int kPmColS = 0, kPmColO = 256;
 constexpr float kPmLazy = 8.f;                   // log2 units
 constexpr int kPmPlanThreads = 1024;
+constexpr int kPmSplitMin = 4;                   // key blocks that a split is worth
+constexpr int kPmMaxSplit = 32;
 constexpr int kPmBins = 256;
 
 struct PromptItem {          // one 256-row tile of one sequence
@@ -61,20 +63,29 @@ struct PromptItem {          // one 256-row tile of one sequence
   int k0;                    // contiguous keys: index of the sequence's first key; paged: the sequence
   int nk;                    // keys of the sequence
   int vis0;                  // keys the tile's first token sees, minus one; token i sees min(nk, vis0 + i + 1)
-  int pad[3];
+  int h;                     // kv head (partials only: the merge reads it here)
+  int pad[2];
 };
 
 struct PromptCtrl {
   int n_items;
   int next;                  // next unit to hand out
-  int q_lo, q_hi;            // rows of q inside sequences: [q_lo, q_hi)
+};
+
+struct PromptSeqs {            // the sequences of a call, as the planner or (direct) every CTA reads them
+  const int32_t *cu_q, *cu_k, *lens;   // lens: paged (keys of each sequence); else cu_k
+  int S, Tq, Tk, tpt, causal;
 };
 
 struct PromptParams {
   CUtensorMap tmQ, tmK, tmV;
   __half* out;
-  const PromptItem* items;
+  PromptItem* items;
   PromptCtrl* ctrl;
+  PromptSeqs seqs;
+  int direct;                  // one unit (or one split of it) per CTA, found by the CTA itself: no planner
+  int nsplit;                  // direct: CTAs that share the keys of a unit; above 1 they emit partials
+  float *part_ml, *part_o;     // [CTA][256][2], [CTA][256][128]
   const int32_t* page_table;   // paged cache: (S, table_stride); null = packed keys
   int page_size, table_stride, page_groups;
   int Tq, Hq, Hkv, G, tpt;     // tpt = tokens per 128-row tile
@@ -84,10 +95,10 @@ struct PromptParams {
 };
 
 struct PromptPlanParams {
-  const int32_t *cu_q, *cu_k, *lens;   // lens: paged (keys of each sequence); else cu_k
+  PromptSeqs seqs;
   PromptItem* items;
   PromptCtrl* ctrl;
-  int S, Tq, Tk, tpt, causal, max_items, first_units;
+  int max_items, first_units;
   int32_t* status;
 };
 
@@ -99,7 +110,7 @@ __device__ __forceinline__ int cost_bin(int nblk) {
 }
 
 // One sequence's queries and keys, clamped into their tensors.
-__device__ __forceinline__ bool prompt_seq(const PromptPlanParams& p, int s, int& q0, int& nq, int& k0, int& nk) {
+__device__ __forceinline__ bool prompt_seq(const PromptSeqs& p, int s, int& q0, int& nq, int& k0, int& nk) {
   bool bad = false;
   auto inside = [&](int v, int hi) {
     if (v < 0 || v > hi) bad = true;
@@ -120,6 +131,19 @@ __device__ __forceinline__ bool prompt_seq(const PromptPlanParams& p, int s, int
   return bad;
 }
 
+// Tile t of a sequence.
+__device__ __forceinline__ PromptItem prompt_item(const PromptSeqs& p, int q0, int nq, int k0, int nk, int t) {
+  const int per = 2 * p.tpt;
+  PromptItem it;
+  it.tok0 = q0 + t * per;
+  it.ntok = min(per, nq - t * per);
+  it.k0 = k0;
+  it.nk = nk;
+  it.vis0 = p.causal ? nk - nq + t * per : nk;
+  it.h = it.pad[0] = it.pad[1] = 0;
+  return it;
+}
+
 __global__ void __launch_bounds__(kPmPlanThreads, 1) prompt_plan_kernel(const PromptPlanParams p) {
   __shared__ int s_start[kPmPlanThreads + 1];
   __shared__ int s_q0[kPmPlanThreads], s_nq[kPmPlanThreads], s_k0[kPmPlanThreads], s_nk[kPmPlanThreads];
@@ -131,14 +155,15 @@ __global__ void __launch_bounds__(kPmPlanThreads, 1) prompt_plan_kernel(const Pr
   if (tid < kPmBins) s_hist[tid] = 0;
   if (tid == 0) s_total = 0;
   pdl_wait();
-  const int per = 2 * p.tpt;
+  const PromptSeqs& sq = p.seqs;
+  const int per = 2 * sq.tpt;
   bool bad = false;
   // Pass 0 counts the tiles of each cost, pass 1 places them, the costly ones first.
   for (int pass = 0; pass < 2; ++pass) {
-    for (int base = 0; base < p.S; base += kPmPlanThreads) {
+    for (int base = 0; base < sq.S; base += kPmPlanThreads) {
       const int s = base + tid;
       int q0 = 0, nq = 0, k0 = 0, nk = 0;
-      if (s < p.S) bad |= prompt_seq(p, s, q0, nq, k0, nk);
+      if (s < sq.S) bad |= prompt_seq(sq, s, q0, nq, k0, nk);
       const int tiles = (nq + per - 1) / per;
       int incl = tiles;
 #pragma unroll
@@ -175,13 +200,7 @@ __global__ void __launch_bounds__(kPmPlanThreads, 1) prompt_plan_kernel(const Pr
           if (s_start[mid] <= i) lo = mid; else hi = mid;
         }
         const int t = i - s_start[lo];
-        PromptItem it;
-        it.tok0 = s_q0[lo] + t * per;
-        it.ntok = min(per, s_nq[lo] - t * per);
-        it.k0 = s_k0[lo];
-        it.nk = s_nk[lo];
-        it.vis0 = p.causal ? it.nk - s_nq[lo] + t * per : it.nk;
-        it.pad[0] = it.pad[1] = it.pad[2] = 0;
+        const PromptItem it = prompt_item(sq, s_q0[lo], s_nq[lo], s_k0[lo], s_nk[lo], t);
         const int seen = min(it.nk, max(0, it.vis0 + it.ntok));
         const int bin = kPmBins - 1 - cost_bin((seen + kPmBK - 1) / kPmBK);
         if (pass == 0) {
@@ -219,11 +238,8 @@ __global__ void __launch_bounds__(kPmPlanThreads, 1) prompt_plan_kernel(const Pr
     }
   }
   if (tid == 0) {
-    const int lo = min(max(p.cu_q[0], 0), p.Tq);
     p.ctrl->n_items = min(s_total, p.max_items);
     p.ctrl->next = p.first_units;
-    p.ctrl->q_lo = lo;
-    p.ctrl->q_hi = max(lo, min(max(p.cu_q[p.S], 0), p.Tq));
     if (s_total > p.max_items) bad = true;      // sequences that overlap: more rows than q has
   }
   if (bad) report(p.status, kStatusBadIndex);
@@ -238,7 +254,7 @@ __device__ __forceinline__ float pm_exp2(float x) {
 struct PromptUnit {          // what warp 8 hands to the others
   PromptItem it;
   int h;                     // kv head; -1: no more units
-  int pad[3];
+  int j0, na, nb;            // first key block of this CTA's share, and how many of it tiles A and B have to see
 };
 
 // Key blocks that 128-row tile t of an item has to see, and how many tokens it holds.
@@ -247,6 +263,18 @@ __device__ __forceinline__ int tile_blocks(const PromptItem& it, int t, int tpt)
   if (tok <= t * tpt) return 0;
   const int seen = min(it.nk, max(0, it.vis0 + tok));
   return (seen + kPmBK - 1) / kPmBK;
+}
+
+// This CTA's share of a unit's key blocks: all of them, or part `sp` of `ns` equal ones of at least kPmSplitMin blocks.
+__device__ __forceinline__ int prompt_parts(int nblk, int nsplit) { return max(1, min(nsplit, nblk / kPmSplitMin)); }
+
+__device__ __forceinline__ void prompt_share(PromptUnit& u, int tpt, int nsplit, int sp) {
+  const int na = tile_blocks(u.it, 0, tpt), nb = tile_blocks(u.it, 1, tpt), nblk = max(na, nb);
+  const int parts = prompt_parts(nblk, nsplit);
+  const int j0 = sp < parts ? (int)((long long)nblk * sp / parts) : nblk, j1 = sp < parts ? (int)((long long)nblk * (sp + 1) / parts) : nblk;
+  u.j0 = j0;
+  u.na = max(0, min(na, j1) - j0);
+  u.nb = max(0, min(nb, j1) - j0);
 }
 
 constexpr int kPmBars = 2 * kPmSlots + 2 * kPmSched + 2 + 2 + 2 + 2 + 2;
@@ -300,6 +328,49 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();
+  if (p.direct) {
+    // This CTA's tile: a scan over the sequences' tile counts by the whole block.  (One CTA of a planner would cost a
+    // launch and its own time before any of these begins.)
+    const int sp = blockIdx.x % p.nsplit, u = blockIdx.x / p.nsplit, want = u / p.Hkv;
+    int* s_warp = reinterpret_cast<int*>(units + 1);
+    if (tid == 0) units[0].h = -1;
+    int before = 0;
+    bool bad = false;
+    for (int base = 0; base < p.seqs.S && before <= want; base += kPmThreads) {
+      int q0 = 0, nq = 0, k0 = 0, nk = 0;
+      if (base + tid < p.seqs.S) bad |= prompt_seq(p.seqs, base + tid, q0, nq, k0, nk);
+      const int tiles = (nq + 2 * p.tpt - 1) / (2 * p.tpt);
+      int incl = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (lane == 31) s_warp[warp] = incl;
+      __syncthreads();
+      int total = 0;
+#pragma unroll
+      for (int w = 0; w < kPmThreads / 32; ++w) {
+        const int v = s_warp[w];
+        if (w < warp) incl += v;
+        total += v;
+      }
+      const int t = want - (before + incl - tiles);
+      if (t >= 0 && t < tiles) {
+        PromptUnit un;
+        un.it = prompt_item(p.seqs, q0, nq, k0, nk, t);
+        un.h = un.it.h = u % p.Hkv;
+        prompt_share(un, p.tpt, p.nsplit, sp);
+        units[0] = un;
+        if (p.nsplit > 1 && sp == 0) p.items[u] = un.it;
+      }
+      before += total;
+      __syncthreads();
+    }
+    if (bad) report(p.status, kStatusBadIndex);
+    if (tid == 0 && p.nsplit > 1 && sp == 0 && units[0].h < 0) p.items[u].ntok = 0;
+    __syncthreads();
+  }
 
   // The registers of a block are fixed at its launch (384 x 168 = 64512): 256 x 216 + 128 x 72 is the same number.  Each
   // side changes its share as the first thing in its own branch; the branches meet again only at the common exit.
@@ -309,7 +380,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
   if (warp == 8) {
     // ------------------------------------------------------------------------------ units and TMA producer
     if (lane == 0) {
-      const int n_units = p.ctrl->n_items * p.Hkv;
+      const int n_units = p.direct ? 0 : p.ctrl->n_items * p.Hkv;
       const uint32_t q_bytes = (uint32_t)(p.tpt * p.G) * 128u * 2u;
       int u = blockIdx.x;
       uint32_t ring = 0, issued_q[2] = {0, 0};
@@ -318,22 +389,23 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
         if (n >= kPmSched && !mbar_wait(&sched_empty[sl], (n / kPmSched - 1) & 1)) { timed_out = true; break; }
         PromptUnit un;
         un.h = -1;
-        if (u < n_units) {
+        if (p.direct) {
+          if (n == 0) un = units[0];                       // found above; there is no second
+        } else if (u < n_units) {
           un.it = p.items[u / p.Hkv];
           un.h = u % p.Hkv;
+          prompt_share(un, p.tpt, 1, 0);
         }
-        units[sl].it = un.it;
-        units[sl].h = un.h;
+        units[sl] = un;
         mbar_arrive(&sched_full[sl]);
         if (un.h < 0) break;
-        const int nt0 = tile_blocks(un.it, 0, p.tpt), nt1 = tile_blocks(un.it, 1, p.tpt);
-        const int nblk = max(nt0, nt1);
+        const int nt0 = un.na, nt1 = un.nb, nblk = max(nt0, nt1);
         for (int i = 0; i < 2 * nblk; ++i, ++ring) {
           const int s = ring % kPmSlots;
           if (ring >= kPmSlots && !mbar_wait(&empty[s], (ring / kPmSlots - 1) & 1)) { timed_out = true; break; }
           const CUtensorMap* tm = (i & 1) ? &p.tmV : &p.tmK;
           uint8_t* dst = sKV + s * kPmTile;
-          const int kb = (i >> 1) * kPmBK;
+          const int kb = (un.j0 + (i >> 1)) * kPmBK;
           mbar_expect_tx(&full[s], kPmTile);
           if (p.page_table == nullptr) {
             tma_load_3d(dst, tm, 0, un.h, un.it.k0 + kb, &full[s]);
@@ -363,7 +435,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
           }
         }
         if (timed_out) break;
-        u = atomicAdd(&p.ctrl->next, 1);
+        if (!p.direct) u = atomicAdd(&p.ctrl->next, 1);
       }
       // no load outlives the CTA: the newest tile of every slot has landed before this warp goes to the exit
       for (uint32_t i = ring > kPmSlots ? ring - kPmSlots : 0; i < ring; ++i) mbar_wait(&full[i % kPmSlots], (i / kPmSlots) & 1);
@@ -391,11 +463,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
         const int sl = n % kPmSched;
         if (!mbar_wait(&sched_full[sl], (n / kPmSched) & 1)) { timed_out = true; break; }
         const int h = units[sl].h;
-        int nt[2] = {0, 0};
-        if (h >= 0) {
-          nt[0] = tile_blocks(units[sl].it, 0, p.tpt);
-          nt[1] = tile_blocks(units[sl].it, 1, p.tpt);
-        }
+        const int nt[2] = {units[sl].na, units[sl].nb};
         mbar_arrive(&sched_empty[sl]);
         if (h < 0) break;
         const int nblk = max(nt[0], nt[1]);
@@ -442,7 +510,8 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
     }
   } else if (warp == 10) {
     // ------------------------------------------------------------------------------ rows outside every sequence
-    const int lo = p.ctrl->q_lo, hi = p.ctrl->q_hi;
+    const int lo = min(max(p.seqs.cu_q[0], 0), p.Tq);
+    const int hi = max(lo, min(max(p.seqs.cu_q[p.seqs.S], 0), p.Tq));
     const size_t row16 = (size_t)p.Hq * (kPmD / 8);       // 16-byte chunks of one token's row
     const size_t n = (size_t)(lo + (p.Tq - hi)) * row16;
     for (size_t e = (size_t)blockIdx.x * 32 + lane; e < n; e += (size_t)gridDim.x * 32) {
@@ -464,11 +533,10 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
       const int sl = n % kPmSched;
       if (!__all_sync(0xffffffffu, mbar_wait(&sched_full[sl], (n / kPmSched) & 1))) { timed_out = true; break; }
       const PromptItem it = units[sl].it;
-      const int h = units[sl].h;
+      const int h = units[sl].h, j0 = units[sl].j0, na = units[sl].na, nb = units[sl].nb;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sched_empty[sl]);
       if (h < 0) break;
-      const int na = tile_blocks(it, 0, p.tpt), nb = tile_blocks(it, 1, p.tpt);
       const int nblk = max(na, nb), mine = t == 0 ? na : nb;
       const int tk = t * p.tpt + tok;                     // token of the row inside the item
       const bool valid = tok < p.tpt && tk < it.ntok;
@@ -480,7 +548,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
       for (int j = 0; j < mine; ++j) {
         if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], n_s++ & 1))) { timed_out = true; break; }
         tc_fence_after();
-        const int kb = j * kPmBK;
+        const int kb = (j0 + j) * kPmBK;
         uint32_t s0[32], s1[32], s2[32], s3[32];
         tmem_ld32(tS, s0);
         tmem_ld32(tS + 32, s1);
@@ -581,6 +649,25 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
         if (!__all_sync(0xffffffffu, mbar_wait(&o_full[t], n_o++ & 1))) { timed_out = true; break; }
         tc_fence_after();
       }
+      if (p.nsplit > 1) {
+        // a share of the keys: the row's maximum, sum and unnormalised output, for the merge
+        const size_t at = (size_t)blockIdx.x * 256 + t * 128 + row;
+        if (valid) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mine > 0 ? m : -INFINITY, l);
+        if (mine > 0) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tO + c * 32, o);
+            tmem_ld_wait();
+            if (!valid) continue;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              reinterpret_cast<uint4*>(p.part_o + at * kPmD + c * 32)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
+        }
+        tc_fence_before();
+        continue;
+      }
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;           // 0: the row saw no key (a NaN stays one)
       __half* dst = p.out + ((size_t)(it.tok0 + tk) * p.Hq + (size_t)h * p.G + g) * kPmD;
 #pragma unroll 1
@@ -616,15 +703,77 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
   }
 }
 
+// Merge of a unit's shares: one warp per row, four columns per lane.
+__global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptParams p) {
+  const int lane = threadIdx.x & 31;
+  const int u = blockIdx.x >> 5, r = (blockIdx.x & 31) * 8 + (threadIdx.x >> 5);       // row of the 256
+  pdl_wait();
+  const PromptItem it = p.items[u];
+  const int t = r >> 7, tok = (r & 127) / p.G, g = (r & 127) - tok * p.G, tk = t * p.tpt + tok;
+  if (tok >= p.tpt || tk >= it.ntok) return;
+  const int parts = prompt_parts(max(tile_blocks(it, 0, p.tpt), tile_blocks(it, 1, p.tpt)), p.nsplit);
+  const size_t at0 = (size_t)u * p.nsplit * 256 + r;
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (lane < parts) ml = *reinterpret_cast<const float2*>(p.part_ml + (at0 + (size_t)lane * 256) * 2);
+  // the maximum leaves a NaN share out of m, but its l is NaN and reaches the sum
+  const float m = warp_max(ml.x);
+  const float w = ml.x == -INFINITY ? 0.f : pm_exp2(ml.x - m);
+  const float l = warp_sum(ml.x == -INFINITY && ml.y == 0.f ? 0.f : w * ml.y);
+  const float scale = l > 0.f || l != l ? 1.f / l : 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) {
+    const float wi = __shfl_sync(0xffffffffu, w, i);
+    if (wi == 0.f) continue;                             // a share that this row sees nothing of may not have been written
+    const float4 v = *reinterpret_cast<const float4*>(p.part_o + (at0 + (size_t)i * 256) * kPmD + lane * 4);
+    o.x += wi * v.x;
+    o.y += wi * v.y;
+    o.z += wi * v.z;
+    o.w += wi * v.w;
+  }
+  uint2 out = make_uint2(0u, 0u);
+  if (scale != 0.f) out = make_uint2(pack2(o.x * scale, o.y * scale, p.bf16), pack2(o.z * scale, o.w * scale, p.bf16));
+  *reinterpret_cast<uint2*>(p.out + ((size_t)(it.tok0 + tk) * p.Hq + (size_t)it.h * p.G + g) * kPmD + lane * 4) = out;
+}
+
 // ------------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------------
 static int prompt_tiles_bound(int Tq, int S, int tpt) {
-  const long long n = (long long)Tq / (2 * tpt) + S;       // each sequence ends with at most one partial tile
+  // ceil(n / per) <= (n - 1) / per + 1 for every sequence that is not empty
+  const long long s = S < Tq ? S : Tq, n = ((long long)Tq - s) / (2 * tpt) + s;
   return n > 0x7fffffffll / 64 ? -1 : (int)n;
 }
 
-static size_t prompt_ws(int n) { return 256 + (size_t)n * sizeof(PromptItem); }
+// How a call is cut.  Up to one unit per SM, every CTA finds its unit itself, and where that leaves half of the SMs or more
+// without one, several CTAs share a unit's keys (few rows over a long cache are bound by how many SMs read it).  Else
+// the planner's list and persistent CTAs.  The batch-invariant mode never splits: how many share depends on the batch.
+struct PromptPlan {
+  int max_items, direct, nsplit, grid;
+  size_t items_bytes, ws_bytes;
+};
+
+static bool prompt_plan(PromptPlan& pl, int S, int Tq, long long keys, int Hkv, int tpt) {
+  pl.max_items = prompt_tiles_bound(Tq, S, tpt);
+  if (pl.max_items < 0 || (long long)pl.max_items * Hkv > 0x3fffffffll) return false;
+  const long long units = (long long)pl.max_items * Hkv;
+  const int sms = sm_count();
+  pl.direct = units <= sms;
+  pl.nsplit = 1;
+  if (pl.direct && !g_batch_invariant && units > 0) {
+    // what prompt_parts can come to for a sequence of all the keys: the bound changes no result, only the scratch
+    const long long most = (keys + kPmBK - 1) / kPmBK / kPmSplitMin;
+    pl.nsplit = (int)(sms / units);
+    if (pl.nsplit > most) pl.nsplit = (int)most;
+    if (pl.nsplit > kPmMaxSplit) pl.nsplit = kPmMaxSplit;
+    if (pl.nsplit < 2) pl.nsplit = 1;
+  }
+  pl.grid = (int)(units < 1 ? 1 : pl.direct ? units * pl.nsplit : sms);
+  const long long listed = pl.direct ? (pl.nsplit > 1 ? units : 0) : pl.max_items;
+  pl.items_bytes = 256 + ((size_t)listed * sizeof(PromptItem) + 255) / 256 * 256;
+  pl.ws_bytes = pl.items_bytes + (pl.nsplit > 1 ? (size_t)pl.grid * 256 * (kPmD + 2) * sizeof(float) : 0);
+  return true;
+}
 
 struct PromptStrides {
   long long tok, head;       // elements
@@ -650,10 +799,10 @@ static int prompt_impl(const void* q, const void* k, const void* v, const int32_
   }
   if (Tk > 0x7fff0000 || Tq > 0x7fff0000) return VMK_E_TOO_LARGE;
   const int G = Hq / Hkv, tpt = 128 / G;
-  const int max_items = prompt_tiles_bound(Tq, S, tpt);
-  if (max_items < 0 || (long long)max_items * Hkv > 0x3fffffffll) return VMK_E_TOO_LARGE;
+  PromptPlan pl;
+  if (!prompt_plan(pl, S, Tq, paged ? (long long)table_stride * page_size : Tk, Hkv, tpt)) return VMK_E_TOO_LARGE;
   if (bad_ptr(ws, 256)) return VMK_E_BADARG;
-  if (ws_bytes < prompt_ws(max_items)) return VMK_E_WORKSPACE;
+  if (ws_bytes < pl.ws_bytes) return VMK_E_WORKSPACE;
 
   PromptParams p;
   memset(&p, 0, sizeof(p));
@@ -681,8 +830,11 @@ static int prompt_impl(const void* q, const void* k, const void* v, const int32_
   }
   p.out = static_cast<__half*>(out);
   p.ctrl = static_cast<PromptCtrl*>(ws);
-  PromptItem* items = reinterpret_cast<PromptItem*>(static_cast<uint8_t*>(ws) + 256);
-  p.items = items;
+  p.items = reinterpret_cast<PromptItem*>(static_cast<uint8_t*>(ws) + 256);
+  p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + pl.items_bytes);
+  p.part_o = p.part_ml + (size_t)pl.grid * 256 * 2;
+  p.direct = pl.direct;
+  p.nsplit = pl.nsplit;
   p.page_table = paged ? page_table : nullptr;
   p.page_size = page_size;
   p.table_stride = table_stride;
@@ -695,52 +847,50 @@ static int prompt_impl(const void* q, const void* k, const void* v, const int32_
   p.sc = kLog2e * 0.08838834764831845f;                    // log2(e) / sqrt(128)
   p.bf16 = bf16;
   p.status = status;
-  const long long units = (long long)max_items * Hkv;
-  const int grid = (int)(units < 1 ? 1 : units < sm_count() ? units : sm_count());
-
-  PromptPlanParams pp;
-  memset(&pp, 0, sizeof(pp));
-  pp.cu_q = cu_q;
-  pp.cu_k = cu_k;
-  pp.lens = lens;
-  pp.items = items;
-  pp.ctrl = p.ctrl;
-  pp.S = S;
-  pp.Tq = Tq;
   const long long cap = (long long)table_stride * page_size;
-  pp.Tk = !keys ? 0 : paged ? (int)(cap > 0x7fff0000ll ? 0x7fff0000ll : cap) : Tk;
-  pp.tpt = tpt;
-  pp.causal = causal;
-  pp.max_items = max_items;
-  pp.first_units = grid;
-  pp.status = status;
+  p.seqs = PromptSeqs{cu_q, cu_k, lens, S, Tq, !keys ? 0 : paged ? (int)(cap > 0x7fff0000ll ? 0x7fff0000ll : cap) : Tk, tpt, causal};
 
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(1);
-  cfg.blockDim = dim3(kPmPlanThreads);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  rc = check_launch(cudaLaunchKernelEx(&cfg, prompt_plan_kernel, pp));
-  if (rc != VMK_OK) return rc;
-  cfg.gridDim = dim3(grid);
+  if (!pl.direct) {
+    PromptPlanParams pp;
+    memset(&pp, 0, sizeof(pp));
+    pp.seqs = p.seqs;
+    pp.items = p.items;
+    pp.ctrl = p.ctrl;
+    pp.max_items = pl.max_items;
+    pp.first_units = pl.grid;
+    pp.status = status;
+    cfg.gridDim = dim3(1);
+    cfg.blockDim = dim3(kPmPlanThreads);
+    rc = check_launch(cudaLaunchKernelEx(&cfg, prompt_plan_kernel, pp));
+    if (rc != VMK_OK) return rc;
+  }
+  cfg.gridDim = dim3(pl.grid);
   cfg.blockDim = dim3(kPmThreads);
   cfg.dynamicSmemBytes = kPmSmem;
-  return check_launch(cudaLaunchKernelEx(&cfg, prompt_kernel, p));
+  rc = check_launch(cudaLaunchKernelEx(&cfg, prompt_kernel, p));
+  if (rc != VMK_OK || pl.nsplit == 1) return rc;
+  cfg.gridDim = dim3(pl.grid / pl.nsplit * 32);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  return check_launch(cudaLaunchKernelEx(&cfg, prompt_merge_kernel, p));
 }
 
 }  // namespace vmk
 
 using namespace vmk;
 
-extern "C" size_t vmk_prompt_workspace_bytes(int S, int Tq, int Hq, int Hkv, int D) {
-  if (S < 0 || Tq < 0 || Hq <= 0 || Hkv <= 0 || D != kPmD || Hq % Hkv != 0 || Hq / Hkv > 16) return 0;
-  const int n = prompt_tiles_bound(Tq, S, 128 / (Hq / Hkv));
-  return n < 0 ? 0 : prompt_ws(n);
+extern "C" size_t vmk_prompt_workspace_bytes(int S, int Tq, long long keys, int Hq, int Hkv, int D) {
+  if (S < 0 || Tq < 0 || keys < 0 || Hq <= 0 || Hkv <= 0 || D != kPmD || Hq % Hkv != 0 || Hq / Hkv > 16) return 0;
+  PromptPlan pl;
+  return prompt_plan(pl, S, Tq, keys, Hkv, 128 / (Hq / Hkv)) ? pl.ws_bytes : 0;
 }
 
 extern "C" int vmk_prompt(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k,

@@ -44,13 +44,12 @@ def kernel(target_probs, tokens, bits, u, draft_probs=None, check=False):
         if t is not None and t.device != dev:
             raise ValueError(f"{name}: expected a tensor on {dev}, got {t.device}")
     lib = _lib.lib()
-    with torch.cuda.device(dev):
-        stream = torch.cuda.current_stream()
-        out = torch.empty(B * (kd + 2), dtype=torch.int32, device=dev)
-        path, count, token = out[:B * kd].view(B, kd), out[B * kd:B * kd + B], out[B * kd + B:]
+    with _lib.on_device(dev):
+        stream = _lib.raw_stream(dev)
+        path, count, token = torch.empty_like(tokens), tokens.new_empty(B), tokens.new_empty(B)
         rc = lib.vmk_accept(_lib.ptr(target_probs), _lib.ptr(draft_probs), _lib.ptr(tokens), _lib.ptr(bits), words, _lib.ptr(u),
                             _lib.ptr(path), _lib.ptr(count), _lib.ptr(token), B, kd, V, DTYPES[dt],
-                            _lib.ptr(_lib.status_word(dev)), stream.cuda_stream)
+                            _lib.ptr(_lib.status_word(dev)), stream)
     _lib.check(rc, "vmk_accept")
     if host:
         path, count, token = path.cpu(), count.cpu(), token.cpu()

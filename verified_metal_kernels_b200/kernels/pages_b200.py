@@ -11,7 +11,7 @@ Pages are given lowest first, to rows in their order.  A pool is a contiguous te
 (layers, pages, heads, page_size, width) or, as dsa's, (pages, page_size, width), of any type whose rows are multiples of
 16 bytes.  Calls on one state belong on one stream; they neither allocate on the host nor synchronise (check=True
 does, and raises on what the device refused: no free page left, an index outside its tensor)."""
-import ctypes
+import struct
 
 import torch
 
@@ -60,7 +60,7 @@ def _pools(pools, dev):
         if shape[-1] * t.element_size() % 16:
             raise ValueError(f"{name}: a position's row must be a multiple of 16 bytes")
         d += [t.data_ptr(), layers, heads, shape[-1] * t.element_size()]
-    return (ctypes.c_int64 * len(d))(*d), pages, page_size
+    return struct.pack(f"{len(d)}q", *d), pages, page_size
 
 
 def _need_refs(refs, pages):
@@ -82,12 +82,12 @@ def reserve(page_table, lens, refs, extra, page_size, check=False):
     need(extra, "extra", torch.int32, shape=(R,))
     _on(dev, extra=extra)
     lib = _lib.lib()
-    with torch.cuda.device(dev):
-        stream = torch.cuda.current_stream()
-        granted = torch.empty(R, dtype=torch.int32, device=dev)
-        ws = _lib.scratch(lib.vmk_pages_workspace_bytes(R, 0, refs.shape[0]), dev)
+    with _lib.on_device(dev):
+        stream = _lib.raw_stream(dev)
+        granted = torch.empty_like(lens)
+        ws = _lib.scratch(lib.vmk_pages_workspace_bytes(R, 0, refs.shape[0]), dev, stream)
         rc = lib.vmk_pages_reserve(_lib.ptr(page_table), R, T, _lib.ptr(lens), _lib.ptr(refs), refs.shape[0], page_size, _lib.ptr(extra),
-                                   _lib.ptr(granted), _lib.ptr(ws), ws.numel(), _lib.ptr(_lib.status_word(dev)), stream.cuda_stream)
+                                   _lib.ptr(granted), _lib.ptr(ws), ws.numel(), _lib.ptr(_lib.status_word(dev)), stream)
     _done(rc, "vmk_pages_reserve", check, dev)
     return granted
 
@@ -121,10 +121,10 @@ def append(k, v, k_pages, v_pages, page_table, cu, lens, check=False):
         src += [t.data_ptr(), t.stride(0) * e if t.shape[0] > 1 else 0, t.stride(1) * e if heads > 1 else 0]
     _on(dev, cu=cu)
     lib = _lib.lib()
-    with torch.cuda.device(dev):
-        stream = torch.cuda.current_stream()
-        rc = lib.vmk_pages_append(pools, (ctypes.c_int64 * 6)(*src), pages, page_size, _lib.ptr(page_table), T, _lib.ptr(cu), _lib.ptr(lens), S,
-                                  k.shape[0], _lib.ptr(_lib.status_word(dev)), stream.cuda_stream)
+    with _lib.on_device(dev):
+        stream = _lib.raw_stream(dev)
+        rc = lib.vmk_pages_append(pools, struct.pack("6q", *src), pages, page_size, _lib.ptr(page_table), T, _lib.ptr(cu), _lib.ptr(lens), S,
+                                  k.shape[0], _lib.ptr(_lib.status_word(dev)), stream)
     _done(rc, "vmk_pages_append", check, dev)
 
 
@@ -141,11 +141,11 @@ def fork(pools, page_table, lens, refs, parents, children, check=False):
     need(children, "children", torch.int32, shape=(F,))
     _on(dev, parents=parents, children=children)
     lib = _lib.lib()
-    with torch.cuda.device(dev):
-        stream = torch.cuda.current_stream()
-        ws = _lib.scratch(lib.vmk_pages_workspace_bytes(R, F, 0), dev)
+    with _lib.on_device(dev):
+        stream = _lib.raw_stream(dev)
+        ws = _lib.scratch(lib.vmk_pages_workspace_bytes(R, F, 0), dev, stream)
         rc = lib.vmk_pages_fork(desc, len(pools), _lib.ptr(page_table), R, T, _lib.ptr(lens), _lib.ptr(refs), pages, page_size, _lib.ptr(parents),
-                                _lib.ptr(children), F, _lib.ptr(ws), ws.numel(), _lib.ptr(_lib.status_word(dev)), stream.cuda_stream)
+                                _lib.ptr(children), F, _lib.ptr(ws), ws.numel(), _lib.ptr(_lib.status_word(dev)), stream)
     _done(rc, "vmk_pages_fork", check, dev)
 
 
@@ -162,10 +162,10 @@ def compact(pools, page_table, lens, refs, path, count, check=False):
     need(count, "count", torch.int32, shape=(R,))
     _on(dev, path=path, count=count)
     lib = _lib.lib()
-    with torch.cuda.device(dev):
-        stream = torch.cuda.current_stream()
+    with _lib.on_device(dev):
+        stream = _lib.raw_stream(dev)
         rc = lib.vmk_pages_compact(desc, len(pools), _lib.ptr(page_table), R, T, _lib.ptr(lens), _lib.ptr(refs), pages, page_size, _lib.ptr(path),
-                                   _lib.ptr(count), kd, _lib.ptr(_lib.status_word(dev)), stream.cuda_stream)
+                                   _lib.ptr(count), kd, _lib.ptr(_lib.status_word(dev)), stream)
     _done(rc, "vmk_pages_compact", check, dev)
 
 
@@ -176,10 +176,10 @@ def free(page_table, lens, refs, keep, page_size, check=False):
     need(keep, "keep", torch.int32, shape=(R,))
     _on(dev, keep=keep)
     lib = _lib.lib()
-    with torch.cuda.device(dev):
-        stream = torch.cuda.current_stream()
+    with _lib.on_device(dev):
+        stream = _lib.raw_stream(dev)
         rc = lib.vmk_pages_free(_lib.ptr(page_table), R, T, _lib.ptr(lens), _lib.ptr(refs), refs.shape[0], page_size, _lib.ptr(keep),
-                                _lib.ptr(_lib.status_word(dev)), stream.cuda_stream)
+                                _lib.ptr(_lib.status_word(dev)), stream)
     _done(rc, "vmk_pages_free", check, dev)
 
 
@@ -194,8 +194,8 @@ def copy(pools, src, dst, check=False):
     need(dst, "dst", torch.int32, shape=tuple(src.shape))
     _on(dev, src=src, dst=dst)
     lib = _lib.lib()
-    with torch.cuda.device(dev):
-        stream = torch.cuda.current_stream()
+    with _lib.on_device(dev):
+        stream = _lib.raw_stream(dev)
         rc = lib.vmk_pages_copy(desc, len(pools), pages, page_size, _lib.ptr(src), _lib.ptr(dst), src.shape[0], _lib.ptr(_lib.status_word(dev)),
-                                stream.cuda_stream)
+                                stream)
     _done(rc, "vmk_pages_copy", check, dev)

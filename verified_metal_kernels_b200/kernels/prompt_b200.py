@@ -3,7 +3,7 @@
 Not one of the reference's three ops, which all decode (reference ops/spec.py:14-25 has the causal chain over a
 cache's last positions, at most 32 of them): it is what fills the caches that they read.  Packed sequences of
 different lengths, causal, grouped heads; contiguous keys or the paged cache of decode_b200.kernel_paged."""
-import ctypes
+import struct
 
 import torch
 
@@ -34,8 +34,10 @@ def _rows(t, name, dtype):
 
 
 def _strides(*tensors):
-    v = [n for t in tensors for n in (t.stride(0), t.stride(1))]
-    return (ctypes.c_int64 * len(v))(*v)
+    """Token and head strides for the C call: null where every tensor is contiguous, else six (two) int64."""
+    if all(t.is_contiguous() for t in tensors):
+        return None
+    return struct.pack(f"{2 * len(tensors)}q", *[n for t in tensors for n in t.stride()[:2]])
 
 
 def _common(q, cu_q):
@@ -71,16 +73,16 @@ def kernel(q, k, v, cu_q, cu_k=None, causal=True, check=False):
     dev = q.device
     _same_device(dev, k=k, v=v, cu_q=cu_q, cu_k=cu_k)
     lib = _lib.lib()
-    with torch.cuda.device(dev):
-        stream = torch.cuda.current_stream()
+    with _lib.on_device(dev):
+        stream = _lib.raw_stream(dev)
         out = torch.empty(q.shape, dtype=dt, device=dev)
-        nbytes = lib.vmk_prompt_workspace_bytes(S, Tq, Hq, Hkv, D) if Hkv else 0
+        nbytes = lib.vmk_prompt_workspace_bytes(S, Tq, Tk, Hq, Hkv, D) if Hkv else 0
         if nbytes == 0:
             raise _lib.VmkError(-2, "prompt: unsupported shape")
-        ws = _lib.scratch(nbytes, dev)
+        ws = _lib.scratch(nbytes, dev, stream)
         rc = lib.vmk_prompt(_lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(cu_q), _lib.ptr(cu_k), _strides(q, k, v),
                             _lib.ptr(out), S, Tq, Tk, Hq, Hkv, D, 1 if causal else 0, 1 if dt == torch.bfloat16 else 0,
-                            _lib.ptr(ws), ws.numel(), _lib.ptr(_lib.status_word(dev)), stream.cuda_stream)
+                            _lib.ptr(ws), ws.numel(), _lib.ptr(_lib.status_word(dev)), stream)
     _lib.check(rc, "vmk_prompt")
     return _lib.finish(out, host, check, dev, "vmk_prompt")
 
@@ -102,16 +104,16 @@ def kernel_paged(q, k_pages, v_pages, page_table, cu_q, lens, causal=True, check
     dev = q.device
     _same_device(dev, k_pages=k_pages, v_pages=v_pages, page_table=page_table, cu_q=cu_q, lens=lens)
     lib = _lib.lib()
-    with torch.cuda.device(dev):
-        stream = torch.cuda.current_stream()
+    with _lib.on_device(dev):
+        stream = _lib.raw_stream(dev)
         out = torch.empty(q.shape, dtype=dt, device=dev)
-        nbytes = lib.vmk_prompt_workspace_bytes(S, Tq, Hq, Hkv, D) if Hkv else 0
+        nbytes = lib.vmk_prompt_workspace_bytes(S, Tq, T * page_size, Hq, Hkv, D) if Hkv else 0
         if nbytes == 0:
             raise _lib.VmkError(-2, "prompt: unsupported shape")
-        ws = _lib.scratch(nbytes, dev)
+        ws = _lib.scratch(nbytes, dev, stream)
         rc = lib.vmk_prompt_paged(_lib.ptr(q), _lib.ptr(k_pages), _lib.ptr(v_pages), _lib.ptr(page_table), pages, page_size,
                                   T, _lib.ptr(cu_q), _lib.ptr(lens), _strides(q), _lib.ptr(out), S, Tq, Hq, Hkv, D,
                                   1 if causal else 0, 1 if dt == torch.bfloat16 else 0, _lib.ptr(ws), ws.numel(),
-                                  _lib.ptr(_lib.status_word(dev)), stream.cuda_stream)
+                                  _lib.ptr(_lib.status_word(dev)), stream)
     _lib.check(rc, "vmk_prompt_paged")
     return _lib.finish(out, False, check, dev, "vmk_prompt_paged")
