@@ -251,6 +251,50 @@ __device__ __forceinline__ float pm_exp2(float x) {
   return y;
 }
 
+__device__ __forceinline__ float pm_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// tcgen05.mma and commit executed by the lanes with `lead` set (one of them) in code that the whole warp runs.
+__device__ __forceinline__ void pm_mma_ss(uint32_t lead, uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                          uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      ".reg .b64 da, db;\n"
+      "setp.ne.b32 p, %6, 0;\n"
+      "setp.ne.b32 q, %7, 0;\n"
+      "mov.b64 da, {%1, %2};\n"
+      "mov.b64 db, {%3, %4};\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n"
+      "}\n" ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void pm_mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      ".reg .b64 db;\n"
+      "setp.ne.b32 p, %5, 0;\n"
+      "setp.ne.b32 q, %6, 0;\n"
+      "mov.b64 db, {%2, %3};\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n"
+      "}\n" ::"r"(d), "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void pm_commit(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n"
+      ".reg .pred q;\n"
+      "setp.ne.b32 q, %1, 0;\n"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+      "}\n" ::"r"(smem_u32(bar)), "r"(lead)
+      : "memory");
+}
+
 struct PromptUnit {          // what warp 8 hands to the others
   PromptItem it;
   int h;                     // kv head; -1: no more units
@@ -277,10 +321,11 @@ __device__ __forceinline__ void prompt_share(PromptUnit& u, int tpt, int nsplit,
   u.nb = max(0, min(nb, j1) - j0);
 }
 
-constexpr int kPmBars = 2 * kPmSlots + 2 * kPmSched + 2 + 2 + 2 + 2 + 2;
+constexpr int kPmBars = 2 * kPmSlots + 2 * kPmSched + 2 + 2 + 2 + 2 + 2 + 2;
 constexpr int kPmSmem = 2 * kPmTile + kPmSlots * kPmTile + kPmBars * 8 + kPmSched * (int)sizeof(PromptUnit) + 16 + 1024;
 static_assert(kPmSmem <= 232448, "shared memory of one CTA");
 
+template <bool BF>
 __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_constant__ PromptParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -293,7 +338,8 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
   uint64_t* q_full = sched_empty + kPmSched;             // [tile] Q tile landed               (TMA bytes)
   uint64_t* q_empty = q_full + 2;                        // [tile] last Q.K^T of a unit done   (MMA commit)
   uint64_t* s_full = q_empty + 2;                        // [tile] scores ready                (MMA commit)
-  uint64_t* p_full = s_full + 2;                         // [tile] P in tensor memory          (4 warps)
+  uint64_t* p_part = s_full + 2;                         // [tile] P of the first 96 keys in tensor memory (4 warps)
+  uint64_t* p_full = p_part + 2;                         // [tile] all of P                    (4 warps)
   uint64_t* o_full = p_full + 2;                         // [tile] last P.V of a unit done     (MMA commit)
   PromptUnit* units = reinterpret_cast<PromptUnit*>(sKV + kPmSlots * kPmTile + kPmBars * 8);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(units + kPmSched);
@@ -312,6 +358,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
       mbar_init(&s_full[t], 1);
+      mbar_init(&p_part[t], 4);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_full[t], 1);
     }
@@ -406,6 +453,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
           const CUtensorMap* tm = (i & 1) ? &p.tmV : &p.tmK;
           uint8_t* dst = sKV + s * kPmTile;
           const int kb = (un.j0 + (i >> 1)) * kPmBK;
+          //TR(4, i >> 1, i & 1)
           mbar_expect_tx(&full[s], kPmTile);
           if (p.page_table == nullptr) {
             tma_load_3d(dst, tm, 0, un.h, un.it.k0 + kb, &full[s]);
@@ -444,69 +492,90 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------------------------ every tcgen05.mma
-    if (lane == 0) {
-      const uint32_t idesc_qk = umma_idesc_16(128, kPmBK, 0, p.bf16), idesc_pv = umma_idesc_16(128, kPmD, 1, p.bf16);
-      const uint32_t hi_k = (uint32_t)(umma_desc_sw128(0) >> 32), lo_k = (uint32_t)umma_desc_sw128(0);
-      const uint32_t q_lo = lo_k + (smem_u32(sQ) >> 4), k_lo = lo_k + (smem_u32(sKV) >> 4);
-      const uint32_t hi_v = (uint32_t)(umma_desc_sw128_mn(0, kPmHalf, 1024) >> 32);
-      const uint32_t v_lo = (uint32_t)umma_desc_sw128_mn(0, kPmHalf, 1024) + (smem_u32(sKV) >> 4);
-      uint32_t ring = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
-      auto qk = [&](int t, uint32_t slot) {
-        const uint32_t d = tmem_base + kPmColS + t * 128, a = q_lo + t * (kPmTile >> 4), b = k_lo + slot * (kPmTile >> 4);
+    // The whole warp runs this code and the instructions themselves are predicated: the descriptors then stay in
+    // uniform registers.  (Inside a one-lane branch every one of them was moved there first, at 75 to 85 issue cycles per
+    // instruction beside the softmax warps of the same scheduler; one M128 N128 K16 takes the pipe 64.)
+    uint32_t lead;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(lead));
+    const uint32_t idesc_qk = umma_idesc_16(128, kPmBK, 0, BF), idesc_pv = umma_idesc_16(128, kPmD, 1, BF);
+    const uint32_t hi_k = (uint32_t)(umma_desc_sw128(0) >> 32), lo_k = (uint32_t)umma_desc_sw128(0);
+    const uint32_t q_lo = lo_k + (smem_u32(sQ) >> 4), k_lo = lo_k + (smem_u32(sKV) >> 4);
+    const uint32_t hi_v = (uint32_t)(umma_desc_sw128_mn(0, kPmHalf, 1024) >> 32);
+    const uint32_t v_lo = (uint32_t)umma_desc_sw128_mn(0, kPmHalf, 1024) + (smem_u32(sKV) >> 4);
+    uint32_t ring = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
+    auto qk = [&](int t, uint32_t slot) {
+      const uint32_t d = tmem_base + kPmColS + t * 128, a = q_lo + t * (kPmTile >> 4), b = k_lo + slot * (kPmTile >> 4);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          umma_f16_w(d, a + (k >> 2) * (kPmHalf >> 4) + (k & 3) * 2, hi_k, b + (k >> 2) * (kPmHalf >> 4) + (k & 3) * 2, hi_k,
-                     idesc_qk, k > 0 ? 1u : 0u);
-        umma_commit(&s_full[t]);
+      for (int k = 0; k < 8; ++k)
+        pm_mma_ss(lead, d, a + (k >> 2) * (kPmHalf >> 4) + (k & 3) * 2, hi_k, b + (k >> 2) * (kPmHalf >> 4) + (k & 3) * 2, hi_k,
+                  idesc_qk, k > 0 ? 1u : 0u);
+      pm_commit(lead, &s_full[t]);
+    };
+    for (uint32_t n = 0; !timed_out; ++n) {
+      const int sl = n % kPmSched;
+      if (!mbar_wait(&sched_full[sl], (n / kPmSched) & 1)) { timed_out = true; break; }
+      const int h = __shfl_sync(0xffffffffu, units[sl].h, 0);
+      const int nt0 = __shfl_sync(0xffffffffu, units[sl].na, 0), nt1 = __shfl_sync(0xffffffffu, units[sl].nb, 0);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sched_empty[sl]);
+      if (h < 0) break;
+      const int nblk = max(nt0, nt1);
+      if (nblk == 0) continue;
+      auto wait_tile = [&](uint32_t i) {
+        if (!mbar_wait(&full[i % kPmSlots], (i / kPmSlots) & 1)) timed_out = true;
       };
-      for (uint32_t n = 0; !timed_out; ++n) {
-        const int sl = n % kPmSched;
-        if (!mbar_wait(&sched_full[sl], (n / kPmSched) & 1)) { timed_out = true; break; }
-        const int h = units[sl].h;
-        const int nt[2] = {units[sl].na, units[sl].nb};
-        mbar_arrive(&sched_empty[sl]);
-        if (h < 0) break;
-        const int nblk = max(nt[0], nt[1]);
-        if (nblk == 0) continue;
-        auto wait_tile = [&](uint32_t i) {
-          if (!mbar_wait(&full[i % kPmSlots], (i / kPmSlots) & 1)) timed_out = true;
-        };
-        wait_tile(ring);                                   // K_0
-        for (int t = 0; t < 2 && !timed_out; ++t) {
-          if (nt[t] == 0) continue;
-          if (!mbar_wait(&q_full[t], n_q[t]++ & 1)) { timed_out = true; break; }
+      wait_tile(ring);                                     // K_0
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int nt = t == 0 ? nt0 : nt1;
+        if (nt == 0 || timed_out) continue;
+        if (!mbar_wait(&q_full[t], n_q[t]++ & 1)) { timed_out = true; continue; }
+        tc_fence_after();
+        qk(t, ring % kPmSlots);
+        if (nt == 1) pm_commit(lead, &q_empty[t]);
+      }
+      if (timed_out) break;
+      pm_commit(lead, &empty[ring % kPmSlots]);
+      for (int j = 0; j < nblk && !timed_out; ++j) {
+        const uint32_t iv = ring + 2 * j + 1, ik = iv + 1;
+        wait_tile(iv);
+        //TR(3, j, 7)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int nt = t == 0 ? nt0 : nt1;
+          if (j >= nt || timed_out) continue;
+          const uint32_t o = tmem_base + kPmColO + t * 128, a = tmem_base + kPmColS + t * 128;
+          const uint32_t b = v_lo + (iv % kPmSlots) * (kPmTile >> 4);
+          //TR(2 + t, j, 0)
+          if (!mbar_wait(&p_part[t], n_p[t] & 1)) { timed_out = true; continue; }
+          //TR(2 + t, j, 1)
           tc_fence_after();
-          qk(t, ring % kPmSlots);
-          if (nt[t] == 1) umma_commit(&q_empty[t]);
+#pragma unroll
+          for (int k = 0; k < 6; ++k) pm_mma_ts(lead, o, a + k * 8, b + k * (2048 >> 4), hi_v, idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
+          if (!mbar_wait(&p_full[t], n_p[t]++ & 1)) { timed_out = true; continue; }
+          //TR(2 + t, j, 2)
+          tc_fence_after();
+#pragma unroll
+          for (int k = 6; k < 8; ++k) pm_mma_ts(lead, o, a + k * 8, b + k * (2048 >> 4), hi_v, idesc_pv, 1u);
+          //TR(2 + t, j, 3)
+          if (j + 1 == nt) {
+            pm_commit(lead, &o_full[t]);
+          } else {
+            wait_tile(ik);
+            if (timed_out) continue;
+            //TR(4, j, 2 + t)
+            qk(t, ik % kPmSlots);
+            //TR(2 + t, j, 4)
+            if (j + 2 == nt) pm_commit(lead, &q_empty[t]);
+          }
         }
         if (timed_out) break;
-        umma_commit(&empty[ring % kPmSlots]);
-        for (int j = 0; j < nblk && !timed_out; ++j) {
-          const uint32_t iv = ring + 2 * j + 1, ik = iv + 1;
-          wait_tile(iv);
-          if (j + 1 < nblk) wait_tile(ik);
-          if (timed_out) break;
-          for (int t = 0; t < 2; ++t) {
-            if (j >= nt[t]) continue;
-            if (!mbar_wait(&p_full[t], n_p[t]++ & 1)) { timed_out = true; break; }
-            tc_fence_after();
-            const uint32_t o = tmem_base + kPmColO + t * 128, a = tmem_base + kPmColS + t * 128;
-            const uint32_t b = v_lo + (iv % kPmSlots) * (kPmTile >> 4);
-#pragma unroll
-            for (int k = 0; k < kPmBK / 16; ++k) umma_f16_ts(o, a + k * 8, b + k * (2048 >> 4), hi_v, idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
-            if (j + 1 == nt[t]) {
-              umma_commit(&o_full[t]);
-            } else {
-              qk(t, ik % kPmSlots);
-              if (j + 2 == nt[t]) umma_commit(&q_empty[t]);
-            }
-          }
-          if (timed_out) break;
-          umma_commit(&empty[iv % kPmSlots]);
-          if (j + 1 < nblk) umma_commit(&empty[ik % kPmSlots]);
-        }
-        ring += 2 * nblk;
+        //TR(3, j, 5)
+        pm_commit(lead, &empty[iv % kPmSlots]);
+        if (j + 1 < nblk) pm_commit(lead, &empty[ik % kPmSlots]);
+        //TR(3, j, 6)
       }
+      ring += 2 * nblk;
     }
   } else if (warp == 10) {
     // ------------------------------------------------------------------------------ rows outside every sequence
@@ -547,34 +616,34 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < mine; ++j) {
         if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], n_s++ & 1))) { timed_out = true; break; }
+        //TR(t, j, 0)
         tc_fence_after();
         const int kb = (j0 + j) * kPmBK;
-        uint32_t s0[32], s1[32], s2[32], s3[32];
-        tmem_ld32(tS, s0);
-        tmem_ld32(tS + 32, s1);
-        tmem_ld32(tS + 64, s2);
-        tmem_ld32(tS + 96, s3);
+        uint32_t sv[128];
+        tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(sv));
+        tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
+        tmem_ld32(tS + 64, *reinterpret_cast<uint32_t(*)[32]>(sv + 64));
+        tmem_ld32(tS + 96, *reinterpret_cast<uint32_t(*)[32]>(sv + 96));
         tmem_ld_wait();
-        if (kb + kPmBK > vis_all) {
+        //TR(t, j, 1)
+        const bool edge = kb + kPmBK > vis_all;
+        if (edge) {
           // a block that the mask or the end of the keys cuts: hidden scores become -inf whatever they were
           const int lim = vis - kb;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (i >= lim) s0[i] = 0xff800000u;
-            if (i + 32 >= lim) s1[i] = 0xff800000u;
-            if (i + 64 >= lim) s2[i] = 0xff800000u;
-            if (i + 96 >= lim) s3[i] = 0xff800000u;
-          }
+          for (int i = 0; i < 128; ++i)
+            if (i >= lim) sv[i] = 0xff800000u;
         }
-        float b0 = -INFINITY, b1 = -INFINITY, b2 = -INFINITY, b3 = -INFINITY;
+        float mx[4];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          b0 = fmaxf(b0, __uint_as_float(s0[i]));
-          b1 = fmaxf(b1, __uint_as_float(s1[i]));
-          b2 = fmaxf(b2, __uint_as_float(s2[i]));
-          b3 = fmaxf(b3, __uint_as_float(s3[i]));
-        }
-        const float bm = fmaxf(fmaxf(b0, b1), fmaxf(b2, b3)) * p.sc;      // the scale is positive: max commutes with it
+        for (int i = 0; i < 4; ++i) mx[i] = pm_max3(__uint_as_float(sv[i]), __uint_as_float(sv[i + 4]), __uint_as_float(sv[i + 8]));
+#pragma unroll
+        for (int i = 12; i < 124; i += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mx[k] = pm_max3(mx[k], __uint_as_float(sv[i + k]), __uint_as_float(sv[i + k + 4]));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(sv[124 + k]));
+        const float bm = fmaxf(pm_max3(mx[0], mx[1], mx[2]), mx[3]) * p.sc;    // the scale is positive: max commutes with it
         const float m_new = fmaxf(m, bm);
         float alpha = 1.f;
         bool rescale = false;
@@ -598,32 +667,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
             tmem_st16(tO + c * 16, o);
           }
         }
-        float ps0 = 0.f, ps1 = 0.f;
-        auto to_p = [&](auto bf_tag, uint32_t (&sc32)[32], int c) {
-          constexpr bool BF = decltype(bf_tag)::value;
-          uint32_t pk[16];
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float a = pm_exp2(fmaf(__uint_as_float(sc32[i]), p.sc, -mu));
-            const float b = pm_exp2(fmaf(__uint_as_float(sc32[i + 1]), p.sc, -mu));
-            ps0 += a;
-            ps1 += b;
-            pk[i >> 1] = BF ? pack_bf16x2(a, b) : pack_half2(a, b);
-          }
-          tmem_st16(tS + c * 16, pk);
-        };
-        if (p.bf16) {
-          to_p(std::true_type{}, s0, 0);
-          to_p(std::true_type{}, s1, 1);
-          to_p(std::true_type{}, s2, 2);
-          to_p(std::true_type{}, s3, 3);
-        } else {
-          to_p(std::false_type{}, s0, 0);
-          to_p(std::false_type{}, s1, 1);
-          to_p(std::false_type{}, s2, 2);
-          to_p(std::false_type{}, s3, 3);
-        }
-        l += ps0 + ps1;
+        //TR(t, j, 2)
         if (kb + kPmBK > it.nk && (t == 0 || j >= na)) {
           // rows of V past the sequence's end are cleared by the tile whose product comes first
           const uint32_t iv = ring + 2 * j + 1;
@@ -636,10 +680,34 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
           }
           fence_proxy_async();
         }
+        // P = 2^(score * scale - m) (exactly 0 for a hidden key: -inf stays -inf), its sum, 16-bit pairs over the scores
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float a = pm_exp2(fmaf(__uint_as_float(sv[c * 32 + 2 * i]), p.sc, -mu));
+            const float b = pm_exp2(fmaf(__uint_as_float(sv[c * 32 + 2 * i + 1]), p.sc, -mu));
+            sum[(i & 1) * 2] += a;
+            sum[(i & 1) * 2 + 1] += b;
+            pk[i] = BF ? pack_bf16x2(a, b) : pack_half2(a, b);
+          }
+          tmem_st16(tS + c * 16, pk);
+          if (c == 2) {                                   // the product of the first 96 keys may begin
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_part[t]);
+          }
+        }
+        //TR(t, j, 3)
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
+        //TR(t, j, 4)
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       }
       if (timed_out) break;
       ring += 2 * nblk;
@@ -682,10 +750,10 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
         for (int i = 0; i < 4; ++i) {
           uint4 w = make_uint4(0u, 0u, 0u, 0u);
           if (mine > 0 && inv != 0.f) {
-            w.x = pack2(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv, p.bf16);
-            w.y = pack2(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv, p.bf16);
-            w.z = pack2(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv, p.bf16);
-            w.w = pack2(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv, p.bf16);
+            w.x = pack2(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv, BF);
+            w.y = pack2(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv, BF);
+            w.z = pack2(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv, BF);
+            w.w = pack2(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv, BF);
           }
           reinterpret_cast<uint4*>(dst + c * 32)[i] = w;
         }
@@ -824,7 +892,8 @@ static int prompt_impl(const void* q, const void* k, const void* v, const int32_
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return VMK_E_LAUNCH;
   if (dev >= 64 || !(configured.load() >> dev & 1)) {
-    const cudaError_t e = cudaFuncSetAttribute(prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPmSmem);
+    cudaError_t e = cudaFuncSetAttribute(prompt_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPmSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(prompt_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPmSmem);
     if (e != cudaSuccess) return check_launch(e);
     if (dev < 64) configured.fetch_or(1ull << dev);
   }
@@ -875,7 +944,7 @@ static int prompt_impl(const void* q, const void* k, const void* v, const int32_
   cfg.gridDim = dim3(pl.grid);
   cfg.blockDim = dim3(kPmThreads);
   cfg.dynamicSmemBytes = kPmSmem;
-  rc = check_launch(cudaLaunchKernelEx(&cfg, prompt_kernel, p));
+  rc = check_launch(bf16 ? cudaLaunchKernelEx(&cfg, prompt_kernel<true>, p) : cudaLaunchKernelEx(&cfg, prompt_kernel<false>, p));
   if (rc != VMK_OK || pl.nsplit == 1) return rc;
   cfg.gridDim = dim3(pl.grid / pl.nsplit * 32);
   cfg.blockDim = dim3(256);
