@@ -634,38 +634,56 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
           for (int i = 0; i < 128; ++i)
             if (i >= lim) sv[i] = 0xff800000u;
         }
-        float mx[4];
+        // P = 2^(score * scale - m) (exactly 0 for a hidden key: -inf stays -inf) and its sum, 32 keys at a time
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t pk[16];
+        auto chunk = [&](int c, float mu, float (&add)[4]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mx[i] = pm_max3(__uint_as_float(sv[i]), __uint_as_float(sv[i + 4]), __uint_as_float(sv[i + 8]));
-#pragma unroll
-        for (int i = 12; i < 124; i += 8)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mx[k] = pm_max3(mx[k], __uint_as_float(sv[i + k]), __uint_as_float(sv[i + k + 4]));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(sv[124 + k]));
-        const float bm = fmaxf(pm_max3(mx[0], mx[1], mx[2]), mx[3]) * p.sc;    // the scale is positive: max commutes with it
-        const float m_new = fmaxf(m, bm);
-        float alpha = 1.f;
-        bool rescale = false;
-        if (m == -INFINITY) {
-          m = m_new;                                     // nothing accumulated for this row yet
-        } else if (m_new > m + kPmLazy) {
-          alpha = pm_exp2(m - m_new);
-          m = m_new;
-          rescale = true;
-        }
-        l *= alpha;
-        const float mu = (m == -INFINITY) ? 0.f : m;
-        if (__any_sync(0xffffffffu, rescale)) {
-#pragma unroll 1
-          for (int c = 0; c < 8; ++c) {
-            uint32_t o[16];
-            tmem_ld16(tO + c * 16, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            tmem_st16(tO + c * 16, o);
+          for (int i = 0; i < 16; ++i) {
+            const float a = pm_exp2(fmaf(__uint_as_float(sv[c * 32 + 2 * i]), p.sc, -mu));
+            const float b = pm_exp2(fmaf(__uint_as_float(sv[c * 32 + 2 * i + 1]), p.sc, -mu));
+            add[(i & 1) * 2] += a;
+            add[(i & 1) * 2 + 1] += b;
+            pk[i] = BF ? pack_bf16x2(a, b) : pack_half2(a, b);
           }
+        };
+        // The first 32 keys go by the maximum of the blocks before: their exponentials need not wait for this block's maximum.
+        // Only where a row's maximum has grown by more than 2^8 (or at a row's first block) they are done again.
+        float mu = (m == -INFINITY) ? 0.f : m;
+        chunk(0, mu, sum);
+        float mx[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx[i] = fmaxf(__uint_as_float(sv[i]), __uint_as_float(sv[i + 8]));
+#pragma unroll
+        for (int i = 16; i < 128; i += 16)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) mx[k] = pm_max3(mx[k], __uint_as_float(sv[i + k]), __uint_as_float(sv[i + k + 8]));
+        mx[0] = pm_max3(mx[0], mx[1], mx[2]);
+        mx[3] = pm_max3(mx[3], mx[4], mx[5]);
+        mx[0] = pm_max3(mx[0], mx[6], mx[7]);
+        const float bm = fmaxf(mx[0], mx[3]) * p.sc;         // the scale is positive: max commutes with it
+        const bool grown = bm > m + kPmLazy;                 // (m is -inf before a row's first visible key)
+        if (__any_sync(0xffffffffu, grown)) {
+          float alpha = 1.f;
+          if (grown) {
+            if (m != -INFINITY) alpha = pm_exp2(m - bm);
+            m = bm;
+          }
+          l *= alpha;
+          if (__any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+              uint32_t o[16];
+              tmem_ld16(tO + c * 16, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st16(tO + c * 16, o);
+            }
+          }
+          mu = (m == -INFINITY) ? 0.f : m;
+          sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
+          chunk(0, mu, sum);
         }
         //TR(t, j, 2)
         if (kb + kPmBK > it.nk && (t == 0 || j >= na)) {
@@ -680,19 +698,10 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
           }
           fence_proxy_async();
         }
-        // P = 2^(score * scale - m) (exactly 0 for a hidden key: -inf stays -inf), its sum, 16-bit pairs over the scores
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        tmem_st16(tS, pk);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float a = pm_exp2(fmaf(__uint_as_float(sv[c * 32 + 2 * i]), p.sc, -mu));
-            const float b = pm_exp2(fmaf(__uint_as_float(sv[c * 32 + 2 * i + 1]), p.sc, -mu));
-            sum[(i & 1) * 2] += a;
-            sum[(i & 1) * 2 + 1] += b;
-            pk[i] = BF ? pack_bf16x2(a, b) : pack_half2(a, b);
-          }
+        for (int c = 1; c < 4; ++c) {
+          chunk(c, mu, sum);
           tmem_st16(tS + c * 16, pk);
           if (c == 2) {                                   // the product of the first 96 keys may begin
             tmem_st_wait();
