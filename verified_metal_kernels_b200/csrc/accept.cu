@@ -12,9 +12,13 @@
 // r(x) off M, which needs no pass.  When no child is left the next token is drawn from r (from p at a leaf, or if r is
 // empty) by the inverse of its cumulative sum at the root's number.
 //
-// Everything is computed in 64 bits: the answers are whole numbers, and an fp32 sum over a vocabulary is off by more
-// than the width of a rare token.  Products and differences are rounded one by one (no fused multiply-add), so a plain
-// 64-bit evaluation gives the same bits but for the order of the sums.  Entries that are NaN, infinite or negative
+// Everything is computed in 64 bits or what equals it: the answers are whole numbers, and an fp32 sum over a vocabulary
+// is off by more than the width of a rare token.  Conversions to fp64 are what a pass over a row is bound by (15 lanes a
+// cycle and SM, 6 elements with both operands converted and the difference taken in fp64), so the difference p - S q is
+// taken in pairs of fp32 numbers without error: with S = Sh + Sl,
+//     t = Sh q rounded, te = Sh q - t (one fused multiply-add), hi = p - t rounded, lo = (p - hi) - t (exact where hi > 0),
+//     p - S q = hi + (lo - te - Sl q), the bracket below 2^-23 of p and rounded at 2^-47;
+// only hi is converted and summed in fp64, the brackets are summed in fp32.  Entries that are NaN, infinite or negative
 // count as 0.
 //
 // Of a request's kd rows only those are read at which a draft is refused or the walk ends; the rest of the walk needs
@@ -25,6 +29,7 @@
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
+#include <atomic>
 #include <cstring>
 
 #include "common.cuh"
@@ -37,6 +42,7 @@ constexpr int kAcThreads = 512;
 constexpr int kAcWarps = kAcThreads / 32;
 constexpr int kAcNodes = VMK_SPEC_MAX_DRAFTS;
 constexpr int kAcCluster = 8;
+static_assert(kAcNodes <= kAcThreads, "one thread per node");
 
 struct AcceptParams {
   const void *p, *q;             // (B, kd, V), q null: drafts without probabilities
@@ -49,12 +55,14 @@ struct AcceptParams {
 };
 
 struct AcceptShared {
-  double p[kAcNodes], q[kAcNodes], u[kAcNodes];
+  float p[kAcNodes], q[kAcNodes], u[kAcNodes];
   int token[kAcNodes], parent[kAcNodes];
   int gone[kAcNodes];            // tokens refused at the current node (drafts without probabilities)
   int path[kAcNodes];
   double warp_sum[kAcWarps];
   double rank_sum[2][kAcCluster];   // every CTA's sum of a pass; alternating, so that one barrier a pass is enough
+  double scan[kAcWarps];
+  int found, positive;
 };
 
 // Sanitised probability: positive and finite, else 0.
@@ -94,19 +102,30 @@ __device__ __forceinline__ void ac_load(AcVec<T>& v, const T* row, int head, int
   }
 }
 
-// Weights of one vector: max(p - S q, 0), or p without the refused tokens.
+struct AcScale {                 // S as two fp32 numbers; 0: q is not taken off
+  float hi, lo;
+};
+
+// Weights max(p - S q, 0) of one vector, or p without the refused tokens, as hi + lo.
 template <typename T, bool HAS_Q>
-__device__ __forceinline__ void ac_weights(double (&w)[AcVec<T>::N], const AcVec<T>& p, const AcVec<T>& q, double S, bool minus_q,
-                                           const int* gone, int n_gone, int e0) {
+__device__ __forceinline__ void ac_weights(float (&hi)[AcVec<T>::N], float (&lo)[AcVec<T>::N], const AcVec<T>& p, const AcVec<T>& q,
+                                           AcScale S, const int* gone, int n_gone, int e0) {
   constexpr int N = AcVec<T>::N;
 #pragma unroll
-  for (int k = 0; k < N; ++k) w[k] = (double)ac_clean(ac_float<T>(p.e[k]));
+  for (int k = 0; k < N; ++k) {
+    hi[k] = ac_clean(ac_float<T>(p.e[k]));
+    lo[k] = 0.f;
+  }
   if (HAS_Q) {
-    if (minus_q) {
+    if (S.hi != 0.f) {
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        const double d = __dsub_rn(w[k], __dmul_rn(S, (double)ac_clean(ac_float<T>(q.e[k]))));
-        w[k] = d > 0.0 ? d : 0.0;
+        const float y = ac_clean(ac_float<T>(q.e[k])), t = __fmul_rn(S.hi, y), te = __fmaf_rn(S.hi, y, -t);
+        const float d = __fsub_rn(hi[k], t), e = __fsub_rn(__fsub_rn(hi[k], d), t);
+        const float r = __fmaf_rn(-S.lo, y, __fsub_rn(e, te));
+        const bool some = d + r > 0.f;
+        hi[k] = some ? d : 0.f;
+        lo[k] = some ? r : 0.f;
       }
     }
   } else {
@@ -114,17 +133,19 @@ __device__ __forceinline__ void ac_weights(double (&w)[AcVec<T>::N], const AcVec
       const int k0 = gone[g] - e0;
 #pragma unroll
       for (int k = 0; k < N; ++k)
-        if (k == k0) w[k] = 0.0;
+        if (k == k0) hi[k] = 0.f;
     }
   }
 }
 
 template <typename T, bool HAS_Q>
-__global__ void __launch_bounds__(kAcThreads) accept_kernel(const AcceptParams a) {
+__global__ void __launch_bounds__(kAcThreads, 2) accept_kernel(const AcceptParams a) {
   constexpr int N = AcVec<T>::N;
   __shared__ AcceptShared sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
+  // (waited for before anything is written into a peer's shared memory: the peer runs by then)
+  if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const int b = blockIdx.x / ranks;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kd = a.kd, V = a.V;
@@ -134,16 +155,20 @@ __global__ void __launch_bounds__(kAcThreads) accept_kernel(const AcceptParams a
   const size_t node0 = (size_t)b * kd;
   if (tid < kd) {
     const uint32_t* words = a.bits + (node0 + tid) * a.words;
-    int parent = -1;
-    for (int w = (tid - 1) >> 5; w >= 0 && parent < 0 && tid > 0; --w) {
-      uint32_t m = w < a.words ? words[w] : 0u;
-      if (w == tid >> 5) m &= (1u << (tid & 31)) - 1u;
-      if (m != 0u) parent = w * 32 + 31 - __clz(m);
-    }
     const int x = a.tokens[node0 + tid];
+    const float u = a.u[node0 + tid];
+    uint32_t m[kAcNodes / 32];
+#pragma unroll
+    for (int w = 0; w < kAcNodes / 32; ++w) m[w] = w < a.words && w * 32 < tid ? words[w] : 0u;
+    int parent = -1;
+#pragma unroll
+    for (int w = 0; w < kAcNodes / 32; ++w) {
+      if (w == tid >> 5) m[w] &= (1u << (tid & 31)) - 1u;
+      if (m[w] != 0u) parent = w * 32 + 31 - __clz(m[w]);
+    }
     const bool inside = x >= 0 && x < V;
     float p = 0.f, q = 0.f;
-    if (tid > 0 && parent >= 0 && inside) {
+    if (parent >= 0 && inside) {
       const size_t at = (node0 + parent) * V + x;
       p = ac_clean(ac_float<T>(static_cast<const T*>(a.p)[at]));
       if (HAS_Q) q = ac_clean(ac_float<T>(static_cast<const T*>(a.q)[at]));
@@ -153,10 +178,11 @@ __global__ void __launch_bounds__(kAcThreads) accept_kernel(const AcceptParams a
     sh.token[tid] = x;
     sh.p[tid] = p;
     sh.q[tid] = q;
-    sh.u[tid] = a.u[node0 + tid];
+    sh.u[tid] = u;
     sh.path[tid] = tid == 0 ? 0 : -1;
   }
-  cluster.sync();                                // and every peer runs before anything is written into its shared memory
+  __syncthreads();
+  if (ranks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
   int mine[kAcNodes / 32];                       // every warp: parents of the nodes lane, lane + 32, ...
 #pragma unroll
@@ -164,41 +190,49 @@ __global__ void __launch_bounds__(kAcThreads) accept_kernel(const AcceptParams a
 
   int cur = 0, n_path = 1, n_gone = 0, passes = 0;
   double S = 0.0, M = 1.0;
-  int head = 0, nvec = 0, seg = 0, seg0 = 0;     // this warp's vectors of the row: [seg0, min(seg0 + seg, nvec))
   const T *prow = nullptr, *qrow = nullptr;
   bool q16 = true;                               // rows of p and q begin at the same place of a 16-byte vector
+  int head = 0, nvec = 0, seg = 0;               // every warp of the cluster has `seg` vectors of the row
+  AcScale scale{0.f, 0.f};
 
   // Sum of the current weights over the row: every CTA's in rank_sum, every warp's of this CTA in warp_sum.
-  auto pass = [&](bool minus_q) -> double {
+  auto pass = [&]() -> double {
     prow = static_cast<const T*>(a.p) + (node0 + cur) * V;
     qrow = HAS_Q ? static_cast<const T*>(a.q) + (node0 + cur) * V : prow;
     q16 = ((reinterpret_cast<uintptr_t>(prow) ^ reinterpret_cast<uintptr_t>(qrow)) & 15) == 0;
     head = (int)((reinterpret_cast<uintptr_t>(prow) & 15) / sizeof(T));
     nvec = (head + V + N - 1) / N;
     seg = (nvec + ranks * kAcWarps - 1) / (ranks * kAcWarps);
-    seg0 = (rank * kAcWarps + warp) * seg;
-    const int end = min(seg0 + seg, nvec);
-    double sum[4] = {0.0, 0.0, 0.0, 0.0};
-    for (int i = seg0 + lane; i < end; i += 4 * 32) {
-      AcVec<T> p[4], q[4];
+    scale.hi = HAS_Q ? (float)S : 0.f;
+    scale.lo = HAS_Q ? (float)(S - (double)scale.hi) : 0.f;
+    const bool minus_q = scale.hi != 0.f;
+    const int first = (rank * kAcWarps + warp) * seg, end = min(first + seg, nvec);
+    double sum[2] = {0.0, 0.0};
+    float low = 0.f;
+    constexpr int U = HAS_Q && sizeof(T) == 2 ? 2 : 4;     // vectors in flight: what 64 registers hold
+    for (int i = first + lane; i < end; i += U * 32) {
+      AcVec<T> p[U], q[U];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < U; ++k) {
         if (i + k * 32 < end) {
           ac_load<T>(p[k], prow, head, V, i + k * 32);
           if (HAS_Q && minus_q) ac_load<T>(q[k], qrow, head, V, i + k * 32, q16);
         }
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < U; ++k) {
         if (i + k * 32 < end) {
-          double w[N];
-          ac_weights<T, HAS_Q>(w, p[k], q[k], S, minus_q, sh.gone, n_gone, (i + k * 32) * N - head);
+          float hi[N], lo[N];
+          ac_weights<T, HAS_Q>(hi, lo, p[k], q[k], scale, sh.gone, n_gone, (i + k * 32) * N - head);
 #pragma unroll
-          for (int e = 0; e < N; ++e) sum[e & 3] += w[e];
+          for (int e = 0; e < N; ++e) {
+            sum[e & 1] += (double)hi[e];
+            if (HAS_Q) low += lo[e];
+          }
         }
       }
     }
-    double t = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    double t = sum[0] + sum[1] + (double)low;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     __syncthreads();                             // readers of the pass before are done with warp_sum
@@ -207,10 +241,11 @@ __global__ void __launch_bounds__(kAcThreads) accept_kernel(const AcceptParams a
     double* mine_sum = &sh.rank_sum[passes & 1][0];
     if (tid < ranks) {
       double all = 0.0;
+#pragma unroll
       for (int w = 0; w < kAcWarps; ++w) all += sh.warp_sum[w];
       *cluster.map_shared_rank(mine_sum + rank, tid) = all;
     }
-    cluster.sync();
+    if (ranks > 1) cluster.sync(); else __syncthreads();
     double total = 0.0;
     for (int r = 0; r < ranks; ++r) total += mine_sum[r];
     ++passes;
@@ -252,7 +287,7 @@ __global__ void __launch_bounds__(kAcThreads) accept_kernel(const AcceptParams a
           moved = true;
         } else if (HAS_Q) {
           S += M;
-          M = pass(true);
+          M = pass();
           T_left = M;
           have_sum = true;
         } else {
@@ -268,17 +303,15 @@ __global__ void __launch_bounds__(kAcThreads) accept_kernel(const AcceptParams a
   }
 
   // ---- the next token
-  bool minus_q = HAS_Q && S > 0.0;
-  if (!have_sum) T_left = pass(minus_q);
-  if (!(T_left > 0.0) && (minus_q || n_gone > 0)) {
-    minus_q = false;                             // the residual is empty: the target itself
+  if (!have_sum) T_left = pass();
+  if (!(T_left > 0.0) && (S > 0.0 || n_gone > 0)) {
+    S = 0.0;                                     // the residual is empty: the target itself
     n_gone = 0;
-    T_left = pass(false);
+    T_left = pass();
   }
-  int token = -1;
-  const double* rank_sum = sh.rank_sum[(passes - 1) & 1];
   if (T_left > 0.0) {
-    const double target = __dmul_rn(sh.u[0], T_left);
+    const double* rank_sum = sh.rank_sum[(passes - 1) & 1];
+    const double target = __dmul_rn((double)sh.u[0], T_left);
     // first CTA, then first warp of it, whose running sum exceeds the target; the last one that has anything if none does
     int owner = -1, last = 0;
     double before = 0.0, before_last = 0.0, run = 0.0;
@@ -300,49 +333,54 @@ __global__ void __launch_bounds__(kAcThreads) accept_kernel(const AcceptParams a
         run += s;
       }
       if (ow < 0) { ow = lw; wb = wbl; }
-      if (ow == warp) {
-        const int end = min(seg0 + seg, nvec);
-        run = wb;
-        int found = -1, positive = -1;
-        for (int i0 = seg0; i0 < end && found < 0; i0 += 32) {
-          const int i = i0 + lane;
-          double w[N];
-#pragma unroll
-          for (int e = 0; e < N; ++e) w[e] = 0.0;
-          if (i < end) {
-            AcVec<T> p, q;
-            ac_load<T>(p, prow, head, V, i);
-            if (HAS_Q && minus_q) ac_load<T>(q, qrow, head, V, i, q16);
-            ac_weights<T, HAS_Q>(w, p, q, S, minus_q, sh.gone, n_gone, i * N - head);
-          }
-          double own = 0.0;
-          int my_last = -1;
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            own += w[e];
-            if (w[e] > 0.0) my_last = i * N - head + e;
-          }
-          double incl = own;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double x = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += x;
-          }
-          double c = run + (incl - own);
-          int hit = -1;
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            c += w[e];
-            if (hit < 0 && w[e] > 0.0 && c > target) hit = i * N - head + e;
-          }
-          const uint32_t any = __ballot_sync(0xffffffffu, hit >= 0), pos = __ballot_sync(0xffffffffu, my_last >= 0);
-          if (any != 0u) found = __shfl_sync(0xffffffffu, hit, __ffs(any) - 1);
-          if (pos != 0u) positive = __shfl_sync(0xffffffffu, my_last, 31 - __clz(pos));
-          run += __shfl_sync(0xffffffffu, incl, 31);
-        }
-        token = found >= 0 ? found : positive;
-        if (lane == 0) a.next[b] = token;
+      // that warp's range, a vector to every thread of the CTA
+      const int first = (rank * kAcWarps + ow) * seg, end = min(first + seg, nvec);
+      if (tid == 0) {
+        sh.found = 0x7fffffff;
+        sh.positive = -1;
       }
+      run = wb;
+      for (int i0 = first; i0 < end; i0 += kAcThreads) {
+        const int i = i0 + tid;
+        double w[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = 0.0;
+        if (i < end) {
+          AcVec<T> p, q;
+          ac_load<T>(p, prow, head, V, i);
+          if (HAS_Q && scale.hi != 0.f) ac_load<T>(q, qrow, head, V, i, q16);
+          float hi[N], lo[N];
+          ac_weights<T, HAS_Q>(hi, lo, p, q, scale, sh.gone, n_gone, i * N - head);
+#pragma unroll
+          for (int e = 0; e < N; ++e) w[e] = (double)hi[e] + (double)lo[e];
+        }
+        double own = 0.0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) own += w[e];
+        double incl = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double x = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += x;
+        }
+        __syncthreads();                         // found is set up; readers of the step before are done with scan
+        if (lane == 31) sh.scan[warp] = incl;
+        __syncthreads();
+        double c = run + (incl - own);
+        for (int x = 0; x < warp; ++x) c += sh.scan[x];
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          c += w[e];
+          if (w[e] > 0.0) {
+            if (c > target) atomicMin(&sh.found, i * N - head + e);
+            atomicMax(&sh.positive, i * N - head + e);
+          }
+        }
+        for (int x = 0; x < kAcWarps; ++x) run += sh.scan[x];
+        __syncthreads();
+        if (sh.found != 0x7fffffff) break;
+      }
+      if (tid == 0) a.next[b] = sh.found != 0x7fffffff ? sh.found : sh.positive;
     }
   } else if (rank == 0 && tid == 0) {
     a.next[b] = -1;
@@ -352,34 +390,57 @@ __global__ void __launch_bounds__(kAcThreads) accept_kernel(const AcceptParams a
     if (tid < kd) a.path[node0 + tid] = sh.path[tid];
     if (tid == 0) a.count[b] = n_path;
   }
-  cluster.sync();                                // nobody leaves while a peer may still write into its shared memory
+  // no barrier at the end: what the peers wrote into this CTA's memory was there at the last pass's, and nothing is
+  // written or read there after it
 }
 
-// CTAs per request: as many as keep all requests resident at two CTAs an SM, with at least 2048 entries each.
-static int accept_cluster(int B, int V) {
-  if (g_batch_invariant) return V >= 4 * 2048 ? 4 : 1;    // by the row alone: the order of the sums must not follow the batch
-  int c = kAcCluster;
-  while (c > 1 && ((long long)B * c > 2ll * sm_count() || V < c * 2048)) c >>= 1;
-  return c;
-}
-
-template <typename T>
-static int accept_launch(const AcceptParams& a, int B, cudaStream_t stream) {
-  const int c = accept_cluster(B, a.V);
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = c;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg;
+static void accept_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], int B, int c, cudaStream_t stream) {
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = c;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3((unsigned)B * c);
   cfg.blockDim = dim3(kAcThreads);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
+}
+
+// CTAs per request: the most (up to 8, with at least 2048 entries each) at which the clusters of all requests are resident
+// together.  (32 requests over 131072 entries: clusters of 8 in one wave, against two waves of the same at one CTA an SM.)
+static int accept_cluster(int B, int V) {
+  if (g_batch_invariant) return V >= 4 * 2048 ? 4 : 1;    // by the row alone: the order of the sums must not follow the batch
+  static std::atomic<int> resident[64][4];                 // clusters of 1 << i CTAs that run together, by device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
+  for (int i = 3; i > 0; --i) {
+    const int c = 1 << i;
+    if (V < c * 2048) continue;
+    int n = resident[dev][i].load();
+    if (n == 0) {
+      cudaLaunchConfig_t cfg;
+      cudaLaunchAttribute attr[2];
+      accept_config(cfg, attr, 1, c, nullptr);
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&n, accept_kernel<float, true>, &cfg) != cudaSuccess || n < 1) {
+        (void)cudaGetLastError();
+        n = 1;
+      }
+      resident[dev][i].store(n);
+    }
+    if (B <= n) return c;
+  }
+  return 1;
+}
+
+template <typename T>
+static int accept_launch(const AcceptParams& a, int B, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  accept_config(cfg, attr, B, accept_cluster(B, a.V), stream);
   return check_launch(a.q != nullptr ? cudaLaunchKernelEx(&cfg, accept_kernel<T, true>, a) : cudaLaunchKernelEx(&cfg, accept_kernel<T, false>, a));
 }
 
