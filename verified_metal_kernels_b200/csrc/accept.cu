@@ -18,8 +18,10 @@
 // taken in pairs of fp32 numbers without error: with S = Sh + Sl,
 //     t = Sh q rounded, te = Sh q - t (one fused multiply-add), hi = p - t rounded, lo = (p - hi) - t (exact where hi > 0),
 //     p - S q = hi + (lo - te - Sl q), the bracket below 2^-23 of p and rounded at 2^-47;
-// only hi is converted and summed in fp64, the brackets are summed in fp32.  Entries that are NaN, infinite or negative
-// count as 0.
+// only hi is converted and summed in fp64, the brackets are summed in fp32.  At the first refusal of a node S is 1 and t is
+// q itself: three subtractions.  A pass over a row that L2 holds is bound by its instructions (20 an element took 4.1 us
+// for 16384 entries a CTA).  Entries that are NaN, infinite or negative count as 0; a vector that has one is found by one
+// comparison of bits and cleaned in a branch of its own.
 //
 // Of a request's kd rows only those are read at which a draft is refused or the walk ends; the rest of the walk needs
 // p and q at (parent, token) of each node, gathered by one thread a node before it begins.  A request is a CLUSTER of
@@ -88,13 +90,30 @@ struct AcVec {
   __device__ AcVec() {}
 };
 
-// A row of V probabilities as 16-byte vectors: rows of an odd length begin inside one.  Vector i holds the elements
-// [i * N - head, (i + 1) * N - head); those outside the row are 0.
+// N entries as floats that are positive and finite or 0.
 template <typename T>
-__device__ __forceinline__ void ac_load(AcVec<T>& v, const T* row, int head, int V, int i, bool aligned = true) {
+__device__ __forceinline__ void ac_floats(float (&f)[AcVec<T>::N], const AcVec<T>& v) {
+  constexpr int N = AcVec<T>::N;
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    f[k] = ac_float<T>(v.e[k]);
+    top = max(top, __float_as_uint(f[k]));
+  }
+  if (top > 0x7f7fffffu) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) f[k] = ac_clean(f[k]);
+  }
+}
+
+// A row of V probabilities as 16-byte vectors: rows of an odd length begin inside one.  Vector i holds the elements
+// [i * N - head, (i + 1) * N - head); those outside the row are 0.  `whole`: the vector lies in the row and `row` has the
+// alignment that head stands for.
+template <typename T>
+__device__ __forceinline__ void ac_load(AcVec<T>& v, const T* row, int head, int V, int i, bool whole) {
   constexpr int N = AcVec<T>::N;
   const int e0 = i * N - head;
-  if (aligned && e0 >= 0 && e0 + N <= V) {
+  if (whole) {
     v.raw = __ldg(reinterpret_cast<const uint4*>(row + e0));
   } else {
 #pragma unroll
@@ -111,21 +130,30 @@ template <typename T, bool HAS_Q>
 __device__ __forceinline__ void ac_weights(float (&hi)[AcVec<T>::N], float (&lo)[AcVec<T>::N], const AcVec<T>& p, const AcVec<T>& q,
                                            AcScale S, const int* gone, int n_gone, int e0) {
   constexpr int N = AcVec<T>::N;
+  ac_floats<T>(hi, p);
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    hi[k] = ac_clean(ac_float<T>(p.e[k]));
-    lo[k] = 0.f;
-  }
+  for (int k = 0; k < N; ++k) lo[k] = 0.f;
   if (HAS_Q) {
     if (S.hi != 0.f) {
+      float y[N];
+      ac_floats<T>(y, q);
+      if (S.hi == 1.f && S.lo == 0.f) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const float y = ac_clean(ac_float<T>(q.e[k])), t = __fmul_rn(S.hi, y), te = __fmaf_rn(S.hi, y, -t);
-        const float d = __fsub_rn(hi[k], t), e = __fsub_rn(__fsub_rn(hi[k], d), t);
-        const float r = __fmaf_rn(-S.lo, y, __fsub_rn(e, te));
-        const bool some = d + r > 0.f;
-        hi[k] = some ? d : 0.f;
-        lo[k] = some ? r : 0.f;
+        for (int k = 0; k < N; ++k) {
+          const float d = __fsub_rn(hi[k], y[k]);
+          lo[k] = d > 0.f ? __fsub_rn(__fsub_rn(hi[k], d), y[k]) : 0.f;
+          hi[k] = fmaxf(d, 0.f);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const float t = __fmul_rn(S.hi, y[k]), te = __fmaf_rn(S.hi, y[k], -t);
+          const float d = __fsub_rn(hi[k], t), e = __fsub_rn(__fsub_rn(hi[k], d), t);
+          const float r = __fmaf_rn(-S.lo, y[k], __fsub_rn(e, te));
+          const bool some = d + r > 0.f;
+          hi[k] = some ? d : 0.f;
+          lo[k] = some ? r : 0.f;
+        }
       }
     }
   } else {
@@ -188,15 +216,65 @@ __global__ void __launch_bounds__(kAcThreads, 2) accept_kernel(const AcceptParam
 #pragma unroll
   for (int w = 0; w < kAcNodes / 32; ++w) mine[w] = w * 32 + lane < kd ? sh.parent[w * 32 + lane] : -1;
 
-  int cur = 0, n_path = 1, n_gone = 0, passes = 0;
+  int cur = 0, last = 0, n_path = 1, n_gone = 0, passes = 0;   // last: the child tried last
   double S = 0.0, M = 1.0;
+  double T_left = 0.0;                           // sum of the weights of the last pass, if it was at this state
+  bool have_sum = false;
   const T *prow = nullptr, *qrow = nullptr;
   bool q16 = true;                               // rows of p and q begin at the same place of a 16-byte vector
   int head = 0, nvec = 0, seg = 0;               // every warp of the cluster has `seg` vectors of the row
   AcScale scale{0.f, 0.f};
 
-  // Sum of the current weights over the row: every CTA's in rank_sum, every warp's of this CTA in warp_sum.
-  auto pass = [&]() -> double {
+  // ---- the walk, the same in every thread of the cluster; one turn per child or pass
+  for (;;) {
+    // the next child of the current node
+    int i = -1;
+#pragma unroll
+    for (int w = kAcNodes / 32 - 1; w >= 0; --w) {
+      const uint32_t kids = __ballot_sync(0xffffffffu, mine[w] == cur && w * 32 + lane > last);
+      if (kids != 0u) i = w * 32 + __ffs(kids) - 1;
+    }
+    if (i >= 0) {
+      last = i;
+      const double p = sh.p[i], q = sh.q[i], u = sh.u[i];
+      double r;
+      bool yes;
+      if (HAS_Q) {
+        r = __dsub_rn(p, __dmul_rn(S, q));
+        yes = r > 0.0 && __dmul_rn(__dmul_rn(u, M), q) < r;
+      } else {
+        r = p;
+        const int x = sh.token[i];
+        for (int g = 0; g < n_gone; ++g)
+          if (sh.gone[g] == x) r = 0.0;
+        yes = r > 0.0 && __dmul_rn(u, M) < r;
+      }
+      if (yes) {
+        cur = i;
+        if (tid == 0) sh.path[n_path] = i;
+        ++n_path;
+        S = 0.0;
+        M = 1.0;
+        n_gone = 0;
+        have_sum = false;
+        continue;
+      }
+      if (!HAS_Q) {
+        M = fmax(__dsub_rn(M, r), 0.0);
+        __syncthreads();                         // nobody is still reading the list
+        if (tid == 0) sh.gone[n_gone] = sh.token[i];
+        ++n_gone;
+        __syncthreads();
+        continue;
+      }
+      S += M;
+    } else if (have_sum) {
+      if (T_left > 0.0 || (S == 0.0 && n_gone == 0)) break;
+      S = 0.0;                                   // the residual is empty: the target itself
+      n_gone = 0;
+    }
+
+    // ---- a pass: the sum of the current weights over the row, every CTA's in rank_sum, every warp's of this CTA in warp_sum
     prow = static_cast<const T*>(a.p) + (node0 + cur) * V;
     qrow = HAS_Q ? static_cast<const T*>(a.q) + (node0 + cur) * V : prow;
     q16 = ((reinterpret_cast<uintptr_t>(prow) ^ reinterpret_cast<uintptr_t>(qrow)) & 15) == 0;
@@ -209,28 +287,44 @@ __global__ void __launch_bounds__(kAcThreads, 2) accept_kernel(const AcceptParam
     const int first = (rank * kAcWarps + warp) * seg, end = min(first + seg, nvec);
     double sum[2] = {0.0, 0.0};
     float low = 0.f;
-    constexpr int U = HAS_Q && sizeof(T) == 2 ? 2 : 4;     // vectors in flight: what 64 registers hold
-    for (int i = first + lane; i < end; i += U * 32) {
+    auto add = [&](const AcVec<T>& p, const AcVec<T>& q, int at) {
+      float hi[N], lo[N];
+      ac_weights<T, HAS_Q>(hi, lo, p, q, scale, sh.gone, n_gone, at * N - head);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        sum[e & 1] += (double)hi[e];
+        if (HAS_Q) low += lo[e];
+      }
+    };
+    // whole vectors first, several in flight; then the row's ends, and rows of q that do not match p's alignment
+    constexpr int U = HAS_Q && sizeof(T) == 2 ? 2 : 4;     // what 64 registers hold
+    const int w0 = q16 ? max(first, head > 0 ? 1 : 0) : end, w1 = q16 ? min(end, (head + V) / N) : end;
+    int v = w0 + lane;
+    for (; v + (U - 1) * 32 < w1; v += U * 32) {
       AcVec<T> p[U], q[U];
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        if (i + k * 32 < end) {
-          ac_load<T>(p[k], prow, head, V, i + k * 32);
-          if (HAS_Q && minus_q) ac_load<T>(q[k], qrow, head, V, i + k * 32, q16);
-        }
+        ac_load<T>(p[k], prow, head, V, v + k * 32, true);
+        if (HAS_Q && minus_q) ac_load<T>(q[k], qrow, head, V, v + k * 32, true);
       }
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        if (i + k * 32 < end) {
-          float hi[N], lo[N];
-          ac_weights<T, HAS_Q>(hi, lo, p[k], q[k], scale, sh.gone, n_gone, (i + k * 32) * N - head);
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            sum[e & 1] += (double)hi[e];
-            if (HAS_Q) low += lo[e];
-          }
-        }
+      for (int k = 0; k < U; ++k) add(p[k], q[k], v + k * 32);
+    }
+    for (; v < w1; v += 32) {
+      AcVec<T> p, q;
+      ac_load<T>(p, prow, head, V, v, true);
+      if (HAS_Q && minus_q) ac_load<T>(q, qrow, head, V, v, true);
+      add(p, q, v);
+    }
+    for (int x = first + lane; x < end; x += 32) {
+      if (x >= w0 && x < w1) {                    // done above: on to the last of them
+        x += (w1 - 1 - x) / 32 * 32;
+        continue;
       }
+      AcVec<T> p, q;
+      ac_load<T>(p, prow, head, V, x, false);
+      if (HAS_Q && minus_q) ac_load<T>(q, qrow, head, V, x, false);
+      add(p, q, x);
     }
     double t = sum[0] + sum[1] + (double)low;
 #pragma unroll
@@ -249,66 +343,11 @@ __global__ void __launch_bounds__(kAcThreads, 2) accept_kernel(const AcceptParam
     double total = 0.0;
     for (int r = 0; r < ranks; ++r) total += mine_sum[r];
     ++passes;
-    return total;
-  };
-
-  // ---- the walk, the same in every thread of the cluster
-  double T_left = 0.0;                           // sum of the weights of the last pass
-  bool have_sum = false;
-  for (;;) {
-    bool moved = false;
-#pragma unroll
-    for (int w = 0; w < kAcNodes / 32; ++w) {
-      uint32_t kids = __ballot_sync(0xffffffffu, !moved && mine[w] == cur);
-      while (kids != 0u && !moved) {
-        const int i = w * 32 + __ffs(kids) - 1;
-        kids &= kids - 1u;
-        const double p = sh.p[i], q = sh.q[i], u = sh.u[i];
-        double r;
-        bool yes;
-        if (HAS_Q) {
-          r = __dsub_rn(p, __dmul_rn(S, q));
-          yes = r > 0.0 && __dmul_rn(__dmul_rn(u, M), q) < r;
-        } else {
-          r = p;
-          const int x = sh.token[i];
-          for (int g = 0; g < n_gone; ++g)
-            if (sh.gone[g] == x) r = 0.0;
-          yes = r > 0.0 && __dmul_rn(u, M) < r;
-        }
-        if (yes) {
-          cur = i;
-          if (tid == 0) sh.path[n_path] = i;
-          ++n_path;
-          S = 0.0;
-          M = 1.0;
-          n_gone = 0;
-          have_sum = false;
-          moved = true;
-        } else if (HAS_Q) {
-          S += M;
-          M = pass();
-          T_left = M;
-          have_sum = true;
-        } else {
-          M = fmax(__dsub_rn(M, r), 0.0);
-          __syncthreads();                       // nobody is still reading the list
-          if (tid == 0) sh.gone[n_gone] = sh.token[i];
-          ++n_gone;
-          __syncthreads();
-        }
-      }
-    }
-    if (!moved) break;
+    T_left = M = total;
+    have_sum = true;
   }
 
   // ---- the next token
-  if (!have_sum) T_left = pass();
-  if (!(T_left > 0.0) && (S > 0.0 || n_gone > 0)) {
-    S = 0.0;                                     // the residual is empty: the target itself
-    n_gone = 0;
-    T_left = pass();
-  }
   if (T_left > 0.0) {
     const double* rank_sum = sh.rank_sum[(passes - 1) & 1];
     const double target = __dmul_rn((double)sh.u[0], T_left);
@@ -347,8 +386,9 @@ __global__ void __launch_bounds__(kAcThreads, 2) accept_kernel(const AcceptParam
         for (int e = 0; e < N; ++e) w[e] = 0.0;
         if (i < end) {
           AcVec<T> p, q;
-          ac_load<T>(p, prow, head, V, i);
-          if (HAS_Q && scale.hi != 0.f) ac_load<T>(q, qrow, head, V, i, q16);
+          const bool whole = i * N - head >= 0 && (i + 1) * N - head <= V;
+          ac_load<T>(p, prow, head, V, i, whole);
+          if (HAS_Q && scale.hi != 0.f) ac_load<T>(q, qrow, head, V, i, whole && q16);
           float hi[N], lo[N];
           ac_weights<T, HAS_Q>(hi, lo, p, q, scale, sh.gone, n_gone, i * N - head);
 #pragma unroll
