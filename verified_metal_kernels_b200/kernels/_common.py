@@ -28,3 +28,11 @@ def stage_in(tensors):
             t = t.to("cuda", non_blocking=True)
         out.append(t)
     return out, any_host
+
+
+def need_on(t, name, dtype, shape, dev):
+    """need(t, name, dtype, shape) on device `dev`, in one look where all is well."""
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == dev and t.is_cuda and t.is_contiguous()):
+        return t
+    need(t, name, dtype, shape=shape)
+    raise ValueError(f"{name}: expected a tensor on {dev}, got {t.device}")

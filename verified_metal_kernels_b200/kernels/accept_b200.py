@@ -5,7 +5,7 @@ it is the step after `spec`, once the target's probabilities of every draft row 
 import torch
 
 from .. import _lib
-from ._common import need, stage_in
+from ._common import need, need_on, stage_in
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
@@ -31,18 +31,15 @@ def kernel(target_probs, tokens, bits, u, draft_probs=None, check=False):
     dt = target_probs.dtype
     need(target_probs, "target_probs", dt, dims=3)
     B, kd, V = target_probs.shape
-    need(tokens, "tokens", torch.int32, shape=(B, kd))
+    dev = target_probs.device
+    need_on(tokens, "tokens", torch.int32, (B, kd), dev)
     if not isinstance(bits, torch.Tensor) or bits.dtype != torch.int32:
         raise TypeError("bits: expected an int32 tensor")
     words = 1 if bits.dim() == 2 else bits.shape[2] if bits.dim() == 3 else 0
-    need(bits, "bits", torch.int32, shape=(B, kd) if bits.dim() == 2 else (B, kd, words))
-    need(u, "u", torch.float32, shape=(B, kd))
+    need_on(bits, "bits", torch.int32, (B, kd) if bits.dim() == 2 else (B, kd, words), dev)
+    need_on(u, "u", torch.float32, (B, kd), dev)
     if draft_probs is not None:
-        need(draft_probs, "draft_probs", dt, shape=(B, kd, V))
-    dev = target_probs.device
-    for name, t in (("tokens", tokens), ("bits", bits), ("u", u), ("draft_probs", draft_probs)):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name}: expected a tensor on {dev}, got {t.device}")
+        need_on(draft_probs, "draft_probs", dt, (B, kd, V), dev)
     lib = _lib.lib()
     with _lib.on_device(dev):
         stream = _lib.raw_stream(dev)

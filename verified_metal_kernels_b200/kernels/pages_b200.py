@@ -16,25 +16,23 @@ import struct
 import torch
 
 from .. import _lib
-from ._common import need
+from ._common import need, need_on
 
 
 def _state(page_table, lens, refs):
     need(page_table, "page_table", torch.int32, dims=2)
     R, T = page_table.shape
-    need(lens, "lens", torch.int32, shape=(R,))
     dev = page_table.device
-    _on(dev, lens=lens)
+    need_on(lens, "lens", torch.int32, (R,), dev)
     if refs is not None:
         need(refs, "refs", torch.int32, dims=1)
-        _on(dev, refs=refs)
+        _on(refs, "refs", dev)
     return R, T, dev
 
 
-def _on(dev, **tensors):
-    for name, t in tensors.items():
-        if t.device != dev:
-            raise ValueError(f"{name}: expected a tensor on {dev}, got {t.device}")
+def _on(t, name, dev):
+    if t.device != dev:
+        raise ValueError(f"{name}: expected a tensor on {dev}, got {t.device}")
 
 
 def _pools(pools, dev):
@@ -43,23 +41,25 @@ def _pools(pools, dev):
         raise ValueError("pools: expected a list of 1 to 8 tensors")
     d, pages, page_size = [], None, None
     for i, t in enumerate(pools):
-        name = f"pools[{i}]"
         if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name}: expected a torch tensor, got {type(t).__name__}")
-        need(t, name, t.dtype)
-        if t.dim() not in (3, 4, 5) or t.numel() == 0:
-            raise ValueError(f"{name}: expected (pages,[heads,]page_size,width) or (layers,pages,heads,page_size,width), got {tuple(t.shape)}")
-        _on(dev, **{name: t})
-        layers = t.shape[0] if t.dim() == 5 else 1
-        shape = t.shape[1:] if t.dim() == 5 else t.shape
-        heads = shape[1] if t.dim() > 3 else 1
+            raise TypeError(f"pools[{i}]: expected a torch tensor, got {type(t).__name__}")
+        if not t.is_cuda or not t.is_contiguous():
+            need(t, f"pools[{i}]", t.dtype)
+        shape = t.shape
+        dims = len(shape)
+        if dims not in (3, 4, 5) or 0 in shape:
+            raise ValueError(f"pools[{i}]: expected (pages,[heads,]page_size,width) or (layers,pages,heads,page_size,width), got {tuple(shape)}")
+        if t.device != dev:
+            _on(t, f"pools[{i}]", dev)
+        layers = shape[0] if dims == 5 else 1
+        n, positions, row = shape[1 if dims == 5 else 0], shape[-2], shape[-1] * t.element_size()
         if pages is None:
-            pages, page_size = shape[0], shape[-2]
-        if (shape[0], shape[-2]) != (pages, page_size):
-            raise ValueError(f"{name}: expected {pages} pages of {page_size} positions, got {shape[0]} of {shape[-2]}")
-        if shape[-1] * t.element_size() % 16:
-            raise ValueError(f"{name}: a position's row must be a multiple of 16 bytes")
-        d += [t.data_ptr(), layers, heads, shape[-1] * t.element_size()]
+            pages, page_size = n, positions
+        if n != pages or positions != page_size:
+            raise ValueError(f"pools[{i}]: expected {pages} pages of {page_size} positions, got {n} of {positions}")
+        if row % 16:
+            raise ValueError(f"pools[{i}]: a position's row must be a multiple of 16 bytes")
+        d += (t.data_ptr(), layers, shape[-3] if dims > 3 else 1, row)
     return struct.pack(f"{len(d)}q", *d), pages, page_size
 
 
@@ -79,8 +79,7 @@ def reserve(page_table, lens, refs, extra, page_size, check=False):
     pages or, where what it and the rows before it need exceeds the free pages (or its table is too short), none, and
     stays as it is.  Returns granted (R,) int32, 1 or 0."""
     R, T, dev = _state(page_table, lens, refs)
-    need(extra, "extra", torch.int32, shape=(R,))
-    _on(dev, extra=extra)
+    need_on(extra, "extra", torch.int32, (R,), dev)
     lib = _lib.lib()
     with _lib.on_device(dev):
         stream = _lib.raw_stream(dev)
@@ -105,26 +104,28 @@ def append(k, v, k_pages, v_pages, page_table, cu, lens, check=False):
     pools, pages, page_size = _pools([k_pages, v_pages], dev)
     if k_pages.dim() == 5 or v_pages.dim() == 5:
         raise ValueError("k_pages, v_pages: expected the pools of one layer")
-    src = []
+    tokens, src = len(k) if isinstance(k, torch.Tensor) and k.dim() else 0, []
     for name, t, pool in (("k", k, k_pages), ("v", v, v_pages)):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name}: expected a torch tensor, got {type(t).__name__}")
-        _on(dev, **{name: t})
-        heads = pool.shape[1] if pool.dim() == 4 else 1
+        want = (tokens, pool.shape[1] if pool.dim() == 4 else 1, pool.shape[-1])
         if t.dtype != pool.dtype:
             raise TypeError(f"{name}: expected dtype {pool.dtype}, got {t.dtype}")
-        if t.dim() != 3 or tuple(t.shape) != (k.shape[0], heads, pool.shape[-1]):
-            raise ValueError(f"{name}: expected shape ({k.shape[0]}, {heads}, {pool.shape[-1]}), got {tuple(t.shape)}")
-        e = t.element_size()
-        if t.numel() and (t.stride(2) != 1 or t.data_ptr() % 16 or any(n > 1 and (s < 0 or s * e % 16) for n, s in zip(t.shape[:2], t.stride()))):
+        if t.shape != want:
+            raise ValueError(f"{name}: expected shape {want}, got {tuple(t.shape)}")
+        if t.device != dev:
+            _on(t, name, dev)
+        e, (by_token, by_head, by_width), at = t.element_size(), t.stride(), t.data_ptr()
+        by_token, by_head = (by_token * e if want[0] > 1 else 0), (by_head * e if want[1] > 1 else 0)
+        if tokens and (by_width != 1 or at % 16 or by_token < 0 or by_head < 0 or by_token % 16 or by_head % 16):
             raise ValueError(f"{name}: expected a 16-byte aligned tensor, its innermost axis contiguous, its strides multiples of 16 bytes")
-        src += [t.data_ptr(), t.stride(0) * e if t.shape[0] > 1 else 0, t.stride(1) * e if heads > 1 else 0]
-    _on(dev, cu=cu)
+        src += (at, by_token, by_head)
+    _on(cu, "cu", dev)
     lib = _lib.lib()
     with _lib.on_device(dev):
         stream = _lib.raw_stream(dev)
         rc = lib.vmk_pages_append(pools, struct.pack("6q", *src), pages, page_size, _lib.ptr(page_table), T, _lib.ptr(cu), _lib.ptr(lens), S,
-                                  k.shape[0], _lib.ptr(_lib.status_word(dev)), stream)
+                                  tokens, _lib.ptr(_lib.status_word(dev)), stream)
     _done(rc, "vmk_pages_append", check, dev)
 
 
@@ -138,8 +139,8 @@ def fork(pools, page_table, lens, refs, parents, children, check=False):
     _need_refs(refs, pages)
     need(parents, "parents", torch.int32, dims=1)
     F = parents.shape[0]
-    need(children, "children", torch.int32, shape=(F,))
-    _on(dev, parents=parents, children=children)
+    need_on(children, "children", torch.int32, (F,), dev)
+    _on(parents, "parents", dev)
     lib = _lib.lib()
     with _lib.on_device(dev):
         stream = _lib.raw_stream(dev)
@@ -158,9 +159,8 @@ def compact(pools, page_table, lens, refs, path, count, check=False):
     _need_refs(refs, pages)
     need(path, "path", torch.int32, dims=2)
     kd = path.shape[1]
-    need(path, "path", torch.int32, shape=(R, kd))
-    need(count, "count", torch.int32, shape=(R,))
-    _on(dev, path=path, count=count)
+    need_on(path, "path", torch.int32, (R, kd), dev)
+    need_on(count, "count", torch.int32, (R,), dev)
     lib = _lib.lib()
     with _lib.on_device(dev):
         stream = _lib.raw_stream(dev)
@@ -173,8 +173,7 @@ def free(page_table, lens, refs, keep, page_size, check=False):
     """Row r keeps its first keep[r] (>= 0) positions; the pages behind them are given back (a page that other rows share
     stays theirs), and their slots become -1.  keep[r] = 0 frees the row, keep[r] >= lens[r] leaves it as it is."""
     R, T, dev = _state(page_table, lens, refs)
-    need(keep, "keep", torch.int32, shape=(R,))
-    _on(dev, keep=keep)
+    need_on(keep, "keep", torch.int32, (R,), dev)
     lib = _lib.lib()
     with _lib.on_device(dev):
         stream = _lib.raw_stream(dev)
@@ -191,8 +190,8 @@ def copy(pools, src, dst, check=False):
     dev = pools[0].device
     desc, pages, page_size = _pools(pools, dev)
     need(src, "src", torch.int32, dims=1)
-    need(dst, "dst", torch.int32, shape=tuple(src.shape))
-    _on(dev, src=src, dst=dst)
+    need_on(dst, "dst", torch.int32, tuple(src.shape), dev)
+    _on(src, "src", dev)
     lib = _lib.lib()
     with _lib.on_device(dev):
         stream = _lib.raw_stream(dev)

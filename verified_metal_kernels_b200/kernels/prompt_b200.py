@@ -8,7 +8,7 @@ import struct
 import torch
 
 from .. import _lib
-from ._common import need, stage_in
+from ._common import need, need_on, stage_in
 
 
 def _rows(t, name, dtype):
@@ -16,6 +16,8 @@ def _rows(t, name, dtype):
     positive multiple of 8 elements (a view of a fused q/k/v projection, for instance)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch tensor, got {type(t).__name__}")
+    if t.dtype is dtype and t.dim() == 3 and t.is_cuda and t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
     if not t.is_cuda:
         raise ValueError(f"{name}: expected a CUDA tensor (the kernels have no CPU path)")
     if t.dtype != dtype:
@@ -69,13 +71,14 @@ def kernel(q, k, v, cu_q, cu_k=None, causal=True, check=False):
     _rows(v, "v", dt)
     if tuple(k.shape) != (Tk, Hkv, D) or v.shape != k.shape:
         raise ValueError(f"k, v: expected shape (keys, kv heads, {D}), got {tuple(k.shape)} and {tuple(v.shape)}")
-    cu_k = cu_q if cu_k is None else need(cu_k, "cu_k", torch.int32, shape=(S + 1,))
     dev = q.device
-    _same_device(dev, k=k, v=v, cu_q=cu_q, cu_k=cu_k)
+    cu_k = cu_q if cu_k is None else need_on(cu_k, "cu_k", torch.int32, (S + 1,), dev)
+    if k.device != dev or v.device != dev or cu_q.device != dev:
+        _same_device(dev, k=k, v=v, cu_q=cu_q)
     lib = _lib.lib()
     with _lib.on_device(dev):
         stream = _lib.raw_stream(dev)
-        out = torch.empty(q.shape, dtype=dt, device=dev)
+        out = q.new_empty(q.shape)
         nbytes = lib.vmk_prompt_workspace_bytes(S, Tq, Tk, Hq, Hkv, D) if Hkv else 0
         if nbytes == 0:
             raise _lib.VmkError(-2, "prompt: unsupported shape")
@@ -97,16 +100,17 @@ def kernel_paged(q, k_pages, v_pages, page_table, cu_q, lens, causal=True, check
     need(v_pages, "v_pages", dt, shape=(pages, Hkv, page_size, D))
     need(page_table, "page_table", torch.int32, dims=2)
     T = page_table.shape[1]
-    need(page_table, "page_table", torch.int32, shape=(S, T))
-    need(lens, "lens", torch.int32, shape=(S,))
+    dev = q.device
+    need_on(page_table, "page_table", torch.int32, (S, T), dev)
+    need_on(lens, "lens", torch.int32, (S,), dev)
     if page_size == 0 or page_size % 64 != 0:
         raise ValueError("page_size must be a multiple of 64")
-    dev = q.device
-    _same_device(dev, k_pages=k_pages, v_pages=v_pages, page_table=page_table, cu_q=cu_q, lens=lens)
+    if k_pages.device != dev or v_pages.device != dev or cu_q.device != dev:
+        _same_device(dev, k_pages=k_pages, v_pages=v_pages, cu_q=cu_q)
     lib = _lib.lib()
     with _lib.on_device(dev):
         stream = _lib.raw_stream(dev)
-        out = torch.empty(q.shape, dtype=dt, device=dev)
+        out = q.new_empty(q.shape)
         nbytes = lib.vmk_prompt_workspace_bytes(S, Tq, T * page_size, Hq, Hkv, D) if Hkv else 0
         if nbytes == 0:
             raise _lib.VmkError(-2, "prompt: unsupported shape")
