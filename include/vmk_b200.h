@@ -270,7 +270,8 @@ VMK_API int vmk_dsa_index_project(const void* x, const void* wq, const void* ww,
  *   so that a chunk of new tokens sees the context before it); causal = 0: all nk.  A query that sees no key gets
  *   zeros, and so do the rows of out outside [cu_q[0], cu_q[S]).  Entries outside their tensor are clamped (status).
  *   strides (6 int64 in HOST memory, nullable): token and head strides in elements of q, k and v (the innermost axis
- *   is contiguous); positive multiples of 8.  Null: C-contiguous.  out is C-contiguous.
+ *   is contiguous); positive multiples of 8.  Null: C-contiguous.  out is C-contiguous and
+ *   32-byte aligned.
  *   Keys of other sequences and behind the last one may hold anything.  A NaN or infinity in v INSIDE a sequence
  *   reaches the rows that see it, and may reach rows before it whose last block of 128 keys holds it.
  * vmk_prompt_paged reads the keys of sequence s from the pages of page_table[s] as vmk_decode_paged does: k_pages,

@@ -26,7 +26,7 @@ def test_c_entry_refuses_before_any_launch(lib):
     for name in ("q", "k", "v", "cu_q", "cu_k", "out", "ws"):
         assert _call(lib, **{name: None}) == -1, name
         assert _call(lib, **{name: 258 if not name.startswith("cu") else 257}) == -1, name
-    assert _call(lib, status=2) == -1
+    assert _call(lib, status=2) == -1 and _call(lib, out=272) == -1
     for name in ("S", "Tq", "Tk"):
         assert _call(lib, **{name: -1}) == -1
     assert _call(lib, Hq=0) == -1 and _call(lib, Hkv=0) == -1 and _call(lib, bf16=2) == -1 and _call(lib, causal=5) == -1

@@ -251,6 +251,11 @@ __device__ __forceinline__ float pm_exp2(float x) {
   return y;
 }
 
+__device__ __forceinline__ void pm_store32(void* dst, const uint32_t (&w)[8]) {      // dst 32-byte aligned
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+               "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
 __device__ __forceinline__ float pm_max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -755,8 +760,12 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
             tmem_ld_wait();
             if (!valid) continue;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              reinterpret_cast<uint4*>(p.part_o + at * kPmD + c * 32)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            for (int i = 0; i < 4; ++i) {
+              uint32_t w[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[e] = o[8 * i + e];
+              pm_store32(p.part_o + at * kPmD + c * 32 + i * 8, w);
+            }
           }
         }
         tc_fence_before();
@@ -764,7 +773,9 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
       }
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;           // 0: the row saw no key (a NaN stays one)
       __half* dst = p.out + ((size_t)(it.tok0 + tk) * p.Hq + (size_t)h * p.G + g) * kPmD;
-#pragma unroll 1
+      // (a thread has a row: 32-byte stores fill whole sectors, which 16-byte ones at twice the number did not: a warp's
+      // store of 32 rows takes the load/store unit 32 cycles whatever its width)
+#pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
         if (mine > 0) {
@@ -773,15 +784,12 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
         }
         if (!valid) continue;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint4 w = make_uint4(0u, 0u, 0u, 0u);
-          if (mine > 0 && inv != 0.f) {
-            w.x = pack2(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv, BF);
-            w.y = pack2(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv, BF);
-            w.z = pack2(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv, BF);
-            w.w = pack2(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv, BF);
-          }
-          reinterpret_cast<uint4*>(dst + c * 32)[i] = w;
+        for (int i = 0; i < 2; ++i) {
+          uint32_t w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            w[e] = mine > 0 && inv != 0.f ? pack2(__uint_as_float(o[16 * i + 2 * e]) * inv, __uint_as_float(o[16 * i + 2 * e + 1]) * inv, BF) : 0u;
+          pm_store32(dst + c * 32 + i * 16, w);
         }
       }
       tc_fence_before();                                  // these loads before the p_full of the next unit
@@ -882,7 +890,7 @@ static int prompt_impl(const void* q, const void* k, const void* v, const int32_
   if (S < 0 || Tq < 0 || Tk < 0 || Hq <= 0 || Hkv <= 0 || (bf16 != 0 && bf16 != 1) || (causal != 0 && causal != 1)) return VMK_E_BADARG;
   if (D != kPmD || Hq % Hkv != 0 || Hq / Hkv > 16) return VMK_E_UNSUPPORTED;
   if (Tq == 0) return VMK_OK;
-  if (bad_ptr(q, 16) || bad_ptr(out, 16) || bad_ptr(cu_q, 4) || (status && bad_ptr(status, 4))) return VMK_E_BADARG;
+  if (bad_ptr(q, 16) || bad_ptr(out, 32) || bad_ptr(cu_q, 4) || (status && bad_ptr(status, 4))) return VMK_E_BADARG;
   const bool keys = paged ? pages > 0 : Tk > 0;
   if (keys && (bad_ptr(k, 16) || bad_ptr(v, 16))) return VMK_E_BADARG;
   if (paged) {
