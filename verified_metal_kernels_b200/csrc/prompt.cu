@@ -434,6 +434,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
     if (lane == 0) {
       const int n_units = p.direct ? 0 : p.ctrl->n_items * p.Hkv;
       const uint32_t q_bytes = (uint32_t)(p.tpt * p.G) * 128u * 2u;
+      const int pool_pages = p.page_groups / p.Hkv;
       int u = blockIdx.x;
       uint32_t ring = 0, issued_q[2] = {0, 0};
       for (uint32_t n = 0;; ++n) {
@@ -452,26 +453,36 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
         mbar_arrive(&sched_full[sl]);
         if (un.h < 0) break;
         const int nt0 = un.na, nt1 = un.nb, nblk = max(nt0, nt1);
-        // Paged keys: group index (page, head) of the two 64-key boxes of a block, looked up one block ahead; a page id outside
-        // the pool reads zeros.
-        auto page_of = [&](int key) {
-          const int pg = key / p.page_size;
-          const int id = pg < p.table_stride ? p.page_table[(size_t)un.it.k0 * p.table_stride + pg] : -1;
-          return id >= 0 && id < p.page_groups / p.Hkv ? id * p.Hkv + un.h : p.page_groups;
+        // Paged keys: a block is two 64-key boxes, each inside one page; page ids are read one block ahead, and positions
+        // are kept by counting (a division for each took this thread longer than a block).
+        int pg = 0, off = 0, id[2] = {-1, -1}, next_id[2] = {-1, -1}, y[2] = {0, 0}, next_y[2] = {0, 0};
+        const int32_t* row = nullptr;
+        auto look = [&]() {
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            next_id[b] = b == 1 && off != 0 ? next_id[0] : pg < p.table_stride ? row[pg] : -1;
+            next_y[b] = off;
+            off += 64;
+            if (off == p.page_size) {
+              off = 0;
+              ++pg;
+            }
+          }
         };
-        int z0 = 0, z1 = 0, next0 = 0, next1 = 0;
         if (p.page_table != nullptr && nblk > 0) {
-          next0 = page_of(un.j0 * kPmBK);
-          next1 = page_of(un.j0 * kPmBK + 64);
+          row = p.page_table + (size_t)un.it.k0 * p.table_stride;
+          pg = un.j0 * kPmBK / p.page_size;
+          off = un.j0 * kPmBK - pg * p.page_size;
+          look();
         }
         for (int i = 0; i < 2 * nblk; ++i, ++ring) {
           if (p.page_table != nullptr && (i & 1) == 0) {
-            z0 = next0;
-            z1 = next1;
-            if (i + 2 < 2 * nblk) {
-              next0 = page_of((un.j0 + (i >> 1) + 1) * kPmBK);
-              next1 = page_of((un.j0 + (i >> 1) + 1) * kPmBK + 64);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              id[b] = next_id[b];
+              y[b] = next_y[b];
             }
+            if (i + 2 < 2 * nblk) look();
           }
           const int s = ring % kPmSlots;
           if (ring >= kPmSlots && !mbar_wait(&empty[s], (ring / kPmSlots - 1) & 1)) { timed_out = true; break; }
@@ -484,12 +495,12 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
             tma_load_3d(dst, tm, 0, un.h, un.it.k0 + kb, &full[s]);
             tma_load_3d(dst + kPmHalf, tm, 64, un.h, un.it.k0 + kb, &full[s]);
           } else {
-            // two 64-key boxes, each inside one page
-            const int y0 = kb % p.page_size, y1 = (kb + 64) % p.page_size;
-            tma_load_3d(dst, tm, 0, y0, z0, &full[s]);
-            tma_load_3d(dst + kPmHalf / 2, tm, 0, y1, z1, &full[s]);
-            tma_load_3d(dst + kPmHalf, tm, 64, y0, z0, &full[s]);
-            tma_load_3d(dst + kPmHalf + kPmHalf / 2, tm, 64, y1, z1, &full[s]);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {                  // a page id outside the pool reads zeros
+              const int z = id[b] >= 0 && id[b] < pool_pages ? id[b] * p.Hkv + un.h : p.page_groups;
+              tma_load_3d(dst + b * (kPmHalf / 2), tm, 0, y[b], z, &full[s]);
+              tma_load_3d(dst + kPmHalf + b * (kPmHalf / 2), tm, 64, y[b], z, &full[s]);
+            }
           }
           if (i == 0) {
             // the queries behind the first keys: the slot of K_0 is free earlier than the Q tiles of the unit before
