@@ -42,6 +42,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kAcThreads = 512;
 constexpr int kAcWarps = kAcThreads / 32;
+static_assert(kAcWarps <= 32, "a lane for every warp");
 constexpr int kAcNodes = VMK_SPEC_MAX_DRAFTS;
 constexpr int kAcCluster = 8;
 static_assert(kAcNodes <= kAcThreads, "one thread per node");
@@ -164,6 +165,22 @@ __device__ __forceinline__ void ac_weights(float (&hi)[AcVec<T>::N], float (&lo)
         if (k == k0) hi[k] = 0.f;
     }
   }
+}
+
+// Lanes hold sums of consecutive ranges (those beyond the last range 0), `start` is what lies before them.  The first range whose
+// running sum exceeds `target`, or the last that has anything; `before`: the running sum where it begins.
+__device__ __forceinline__ int ac_pick(double s, double start, double target, double& before) {
+  const int lane = threadIdx.x & 31;
+  double incl = s;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double x = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += x;
+  }
+  const uint32_t over = __ballot_sync(0xffffffffu, s > 0.0 && start + incl > target), some = __ballot_sync(0xffffffffu, s > 0.0);
+  const int i = over != 0u ? __ffs(over) - 1 : some != 0u ? 31 - __clz(some) : 0;
+  before = start + __shfl_sync(0xffffffffu, incl - s, i);
+  return i;
 }
 
 template <typename T, bool HAS_Q>
@@ -333,11 +350,11 @@ __global__ void __launch_bounds__(kAcThreads, 2) accept_kernel(const AcceptParam
     if (lane == 0) sh.warp_sum[warp] = t;
     __syncthreads();
     double* mine_sum = &sh.rank_sum[passes & 1][0];
-    if (tid < ranks) {
-      double all = 0.0;
+    if (warp == 0) {
+      double all = lane < kAcWarps ? sh.warp_sum[lane] : 0.0;
 #pragma unroll
-      for (int w = 0; w < kAcWarps; ++w) all += sh.warp_sum[w];
-      *cluster.map_shared_rank(mine_sum + rank, tid) = all;
+      for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+      if (lane < ranks) *cluster.map_shared_rank(mine_sum + rank, lane) = all;
     }
     if (ranks > 1) cluster.sync(); else __syncthreads();
     double total = 0.0;
@@ -352,33 +369,17 @@ __global__ void __launch_bounds__(kAcThreads, 2) accept_kernel(const AcceptParam
     const double* rank_sum = sh.rank_sum[(passes - 1) & 1];
     const double target = __dmul_rn((double)sh.u[0], T_left);
     // first CTA, then first warp of it, whose running sum exceeds the target; the last one that has anything if none does
-    int owner = -1, last = 0;
-    double before = 0.0, before_last = 0.0, run = 0.0;
-    for (int r = 0; r < ranks; ++r) {
-      const double s = rank_sum[r];
-      if (s > 0.0) { last = r; before_last = run; }
-      if (owner < 0 && s > 0.0 && run + s > target) { owner = r; before = run; }
-      run += s;
-    }
-    if (owner < 0) { owner = last; before = before_last; }
+    double before, wb;
+    const int owner = ac_pick(lane < ranks ? rank_sum[lane] : 0.0, 0.0, target, before);
     if (owner == rank) {
-      int ow = -1, lw = 0;
-      double wb = 0.0, wbl = 0.0;
-      run = before;
-      for (int w = 0; w < kAcWarps; ++w) {
-        const double s = sh.warp_sum[w];
-        if (s > 0.0) { lw = w; wbl = run; }
-        if (ow < 0 && s > 0.0 && run + s > target) { ow = w; wb = run; }
-        run += s;
-      }
-      if (ow < 0) { ow = lw; wb = wbl; }
+      const int ow = ac_pick(lane < kAcWarps ? sh.warp_sum[lane] : 0.0, before, target, wb);
       // that warp's range, a vector to every thread of the CTA
       const int first = (rank * kAcWarps + ow) * seg, end = min(first + seg, nvec);
       if (tid == 0) {
         sh.found = 0x7fffffff;
         sh.positive = -1;
       }
-      run = wb;
+      double run = wb;
       for (int i0 = first; i0 < end; i0 += kAcThreads) {
         const int i = i0 + tid;
         double w[N];
@@ -406,8 +407,15 @@ __global__ void __launch_bounds__(kAcThreads, 2) accept_kernel(const AcceptParam
         __syncthreads();                         // found is set up; readers of the step before are done with scan
         if (lane == 31) sh.scan[warp] = incl;
         __syncthreads();
-        double c = run + (incl - own);
-        for (int x = 0; x < warp; ++x) c += sh.scan[x];
+        // warps before this one, and all of them: a sum over lanes each
+        double part = lane < kAcWarps ? sh.scan[lane] : 0.0, mine_before = lane < warp ? part : 0.0;
+#pragma unroll
+        for (int o = kAcWarps / 2; o > 0; o >>= 1) {
+          part += __shfl_xor_sync(0xffffffffu, part, o);
+          mine_before += __shfl_xor_sync(0xffffffffu, mine_before, o);
+        }
+        part = __shfl_sync(0xffffffffu, part, 0);
+        double c = run + __shfl_sync(0xffffffffu, mine_before, 0) + (incl - own);
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           c += w[e];
@@ -416,7 +424,7 @@ __global__ void __launch_bounds__(kAcThreads, 2) accept_kernel(const AcceptParam
             atomicMax(&sh.positive, i * N - head + e);
           }
         }
-        for (int x = 0; x < kAcWarps; ++x) run += sh.scan[x];
+        run += part;
         __syncthreads();
         if (sh.found != 0x7fffffff) break;
       }
