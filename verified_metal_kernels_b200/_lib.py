@@ -140,40 +140,6 @@ _workspace = Workspace()
 _status = {}
 
 
-class _Here:
-    """What on_device returns where the device is the current one already."""
-
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_here = _Here()
-
-
-def on_device(device):
-    """`with torch.cuda.device(device)`, at no cost where it is the current one."""
-    import torch
-    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-def raw_stream(device):
-    """Handle of torch's current stream on `device` (an integer; no Stream object is built)."""
-    import torch
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-def scratch(nbytes, device, stream_id):
-    """Scratch of a call that is made while `device` is the current one.  Under stream capture it is the graph's own (from
-    the graph's memory pool), so that captured graphs do not share it, nor lose it when a larger one takes its place."""
-    import torch
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
-    return _workspace.get(nbytes, device, stream_id)
-
-
 def workspace(nbytes, device, stream_id):
     return _workspace.get(nbytes, device, stream_id)
 

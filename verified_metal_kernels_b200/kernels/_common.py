@@ -1,6 +1,8 @@
 """Argument checks shared by the kernel modules."""
 import torch
 
+from .. import _lib
+
 
 def need(t, name, dtype, shape=None, dims=None):
     if not isinstance(t, torch.Tensor):
@@ -36,3 +38,24 @@ def need_on(t, name, dtype, shape, dev):
         return t
     need(t, name, dtype, shape=shape)
     raise ValueError(f"{name}: expected a tensor on {dev}, got {t.device}")
+
+
+def elsewhere(dev):
+    """Whether `dev` is not the current device: the caller then makes it so and calls itself again (a `with` that does
+    nothing costs as much as a check)."""
+    return torch._C._cuda_getDevice() != dev.index
+
+
+def handles(dev):
+    """Torch's current stream on `dev` as an integer (no Stream object is built) and the address of the device's status word."""
+    return torch._C._cuda_getCurrentRawStream(dev.index), _lib.status_word(dev).data_ptr()
+
+
+def scratch(nbytes, dev, stream):
+    """Scratch of a call made while `dev` is the current device: address and size.  Under stream capture it is the graph's
+    own (from the graph's memory pool), so that captured graphs do not share it, nor lose it when a larger one takes its place."""
+    if torch._C._cuda_isCurrentStreamCapturing():
+        t = torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
+    else:
+        t = _lib.workspace(nbytes, dev, stream)
+    return t.data_ptr(), t.numel()

@@ -5,7 +5,7 @@ it is the step after `spec`, once the target's probabilities of every draft row 
 import torch
 
 from .. import _lib
-from ._common import need, need_on, stage_in
+from ._common import elsewhere, handles, need, need_on, stage_in
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
@@ -41,12 +41,14 @@ def kernel(target_probs, tokens, bits, u, draft_probs=None, check=False):
     if draft_probs is not None:
         need_on(draft_probs, "draft_probs", dt, (B, kd, V), dev)
     lib = _lib.lib()
-    with _lib.on_device(dev):
-        stream = _lib.raw_stream(dev)
-        path, count, token = torch.empty_like(tokens), tokens.new_empty(B), tokens.new_empty(B)
-        rc = lib.vmk_accept(_lib.ptr(target_probs), _lib.ptr(draft_probs), _lib.ptr(tokens), _lib.ptr(bits), words, _lib.ptr(u),
-                            _lib.ptr(path), _lib.ptr(count), _lib.ptr(token), B, kd, V, DTYPES[dt],
-                            _lib.ptr(_lib.status_word(dev)), stream)
+    if elsewhere(dev):
+        with torch.cuda.device(dev):
+            return kernel(target_probs, tokens, bits, u, draft_probs, check)
+    stream, status = handles(dev)
+    path, count, token = torch.empty_like(tokens), tokens.new_empty(B), tokens.new_empty(B)
+    rc = lib.vmk_accept(target_probs.data_ptr(), _lib.ptr(draft_probs), tokens.data_ptr(), bits.data_ptr(), words, u.data_ptr(),
+                        path.data_ptr(), count.data_ptr(), token.data_ptr(), B, kd, V, DTYPES[dt],
+                        status, stream)
     _lib.check(rc, "vmk_accept")
     if host:
         path, count, token = path.cpu(), count.cpu(), token.cpu()

@@ -16,7 +16,7 @@ import struct
 import torch
 
 from .. import _lib
-from ._common import need, need_on
+from ._common import elsewhere, handles, need, need_on, scratch
 
 
 def _state(page_table, lens, refs):
@@ -81,12 +81,14 @@ def reserve(page_table, lens, refs, extra, page_size, check=False):
     R, T, dev = _state(page_table, lens, refs)
     need_on(extra, "extra", torch.int32, (R,), dev)
     lib = _lib.lib()
-    with _lib.on_device(dev):
-        stream = _lib.raw_stream(dev)
-        granted = torch.empty_like(lens)
-        ws = _lib.scratch(lib.vmk_pages_workspace_bytes(R, 0, refs.shape[0]), dev, stream)
-        rc = lib.vmk_pages_reserve(_lib.ptr(page_table), R, T, _lib.ptr(lens), _lib.ptr(refs), refs.shape[0], page_size, _lib.ptr(extra),
-                                   _lib.ptr(granted), _lib.ptr(ws), ws.numel(), _lib.ptr(_lib.status_word(dev)), stream)
+    if elsewhere(dev):
+        with torch.cuda.device(dev):
+            return reserve(page_table, lens, refs, extra, page_size, check)
+    stream, status = handles(dev)
+    granted = torch.empty_like(lens)
+    ws = scratch(lib.vmk_pages_workspace_bytes(R, 0, refs.shape[0]), dev, stream)
+    rc = lib.vmk_pages_reserve(page_table.data_ptr(), R, T, lens.data_ptr(), refs.data_ptr(), refs.shape[0], page_size, extra.data_ptr(),
+                               granted.data_ptr(), *ws, status, stream)
     _done(rc, "vmk_pages_reserve", check, dev)
     return granted
 
@@ -122,10 +124,12 @@ def append(k, v, k_pages, v_pages, page_table, cu, lens, check=False):
         src += (at, by_token, by_head)
     _on(cu, "cu", dev)
     lib = _lib.lib()
-    with _lib.on_device(dev):
-        stream = _lib.raw_stream(dev)
-        rc = lib.vmk_pages_append(pools, struct.pack("6q", *src), pages, page_size, _lib.ptr(page_table), T, _lib.ptr(cu), _lib.ptr(lens), S,
-                                  tokens, _lib.ptr(_lib.status_word(dev)), stream)
+    if elsewhere(dev):
+        with torch.cuda.device(dev):
+            return append(k, v, k_pages, v_pages, page_table, cu, lens, check)
+    stream, status = handles(dev)
+    rc = lib.vmk_pages_append(pools, struct.pack("6q", *src), pages, page_size, page_table.data_ptr(), T, cu.data_ptr(), lens.data_ptr(), S,
+                              tokens, status, stream)
     _done(rc, "vmk_pages_append", check, dev)
 
 
@@ -142,11 +146,13 @@ def fork(pools, page_table, lens, refs, parents, children, check=False):
     need_on(children, "children", torch.int32, (F,), dev)
     _on(parents, "parents", dev)
     lib = _lib.lib()
-    with _lib.on_device(dev):
-        stream = _lib.raw_stream(dev)
-        ws = _lib.scratch(lib.vmk_pages_workspace_bytes(R, F, 0), dev, stream)
-        rc = lib.vmk_pages_fork(desc, len(pools), _lib.ptr(page_table), R, T, _lib.ptr(lens), _lib.ptr(refs), pages, page_size, _lib.ptr(parents),
-                                _lib.ptr(children), F, _lib.ptr(ws), ws.numel(), _lib.ptr(_lib.status_word(dev)), stream)
+    if elsewhere(dev):
+        with torch.cuda.device(dev):
+            return fork(pools, page_table, lens, refs, parents, children, check)
+    stream, status = handles(dev)
+    ws = scratch(lib.vmk_pages_workspace_bytes(R, F, 0), dev, stream)
+    rc = lib.vmk_pages_fork(desc, len(pools), page_table.data_ptr(), R, T, lens.data_ptr(), refs.data_ptr(), pages, page_size, parents.data_ptr(),
+                            children.data_ptr(), F, *ws, status, stream)
     _done(rc, "vmk_pages_fork", check, dev)
 
 
@@ -162,10 +168,12 @@ def compact(pools, page_table, lens, refs, path, count, check=False):
     need_on(path, "path", torch.int32, (R, kd), dev)
     need_on(count, "count", torch.int32, (R,), dev)
     lib = _lib.lib()
-    with _lib.on_device(dev):
-        stream = _lib.raw_stream(dev)
-        rc = lib.vmk_pages_compact(desc, len(pools), _lib.ptr(page_table), R, T, _lib.ptr(lens), _lib.ptr(refs), pages, page_size, _lib.ptr(path),
-                                   _lib.ptr(count), kd, _lib.ptr(_lib.status_word(dev)), stream)
+    if elsewhere(dev):
+        with torch.cuda.device(dev):
+            return compact(pools, page_table, lens, refs, path, count, check)
+    stream, status = handles(dev)
+    rc = lib.vmk_pages_compact(desc, len(pools), page_table.data_ptr(), R, T, lens.data_ptr(), refs.data_ptr(), pages, page_size, path.data_ptr(),
+                               count.data_ptr(), kd, status, stream)
     _done(rc, "vmk_pages_compact", check, dev)
 
 
@@ -175,10 +183,12 @@ def free(page_table, lens, refs, keep, page_size, check=False):
     R, T, dev = _state(page_table, lens, refs)
     need_on(keep, "keep", torch.int32, (R,), dev)
     lib = _lib.lib()
-    with _lib.on_device(dev):
-        stream = _lib.raw_stream(dev)
-        rc = lib.vmk_pages_free(_lib.ptr(page_table), R, T, _lib.ptr(lens), _lib.ptr(refs), refs.shape[0], page_size, _lib.ptr(keep),
-                                _lib.ptr(_lib.status_word(dev)), stream)
+    if elsewhere(dev):
+        with torch.cuda.device(dev):
+            return free(page_table, lens, refs, keep, page_size, check)
+    stream, status = handles(dev)
+    rc = lib.vmk_pages_free(page_table.data_ptr(), R, T, lens.data_ptr(), refs.data_ptr(), refs.shape[0], page_size, keep.data_ptr(),
+                            status, stream)
     _done(rc, "vmk_pages_free", check, dev)
 
 
@@ -193,8 +203,10 @@ def copy(pools, src, dst, check=False):
     need_on(dst, "dst", torch.int32, tuple(src.shape), dev)
     _on(src, "src", dev)
     lib = _lib.lib()
-    with _lib.on_device(dev):
-        stream = _lib.raw_stream(dev)
-        rc = lib.vmk_pages_copy(desc, len(pools), pages, page_size, _lib.ptr(src), _lib.ptr(dst), src.shape[0], _lib.ptr(_lib.status_word(dev)),
-                                stream)
+    if elsewhere(dev):
+        with torch.cuda.device(dev):
+            return copy(pools, src, dst, check)
+    stream, status = handles(dev)
+    rc = lib.vmk_pages_copy(desc, len(pools), pages, page_size, src.data_ptr(), dst.data_ptr(), src.shape[0], status,
+                            stream)
     _done(rc, "vmk_pages_copy", check, dev)

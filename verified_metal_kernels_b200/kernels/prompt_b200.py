@@ -8,7 +8,7 @@ import struct
 import torch
 
 from .. import _lib
-from ._common import need, need_on, stage_in
+from ._common import elsewhere, handles, need, need_on, scratch, stage_in
 
 
 def _rows(t, name, dtype):
@@ -76,16 +76,18 @@ def kernel(q, k, v, cu_q, cu_k=None, causal=True, check=False):
     if k.device != dev or v.device != dev or cu_q.device != dev:
         _same_device(dev, k=k, v=v, cu_q=cu_q)
     lib = _lib.lib()
-    with _lib.on_device(dev):
-        stream = _lib.raw_stream(dev)
-        out = q.new_empty(q.shape)
-        nbytes = lib.vmk_prompt_workspace_bytes(S, Tq, Tk, Hq, Hkv, D) if Hkv else 0
-        if nbytes == 0:
-            raise _lib.VmkError(-2, "prompt: unsupported shape")
-        ws = _lib.scratch(nbytes, dev, stream)
-        rc = lib.vmk_prompt(_lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(cu_q), _lib.ptr(cu_k), _strides(q, k, v),
-                            _lib.ptr(out), S, Tq, Tk, Hq, Hkv, D, 1 if causal else 0, 1 if dt == torch.bfloat16 else 0,
-                            _lib.ptr(ws), ws.numel(), _lib.ptr(_lib.status_word(dev)), stream)
+    if elsewhere(dev):
+        with torch.cuda.device(dev):
+            return kernel(q, k, v, cu_q, cu_k, causal, check)
+    stream, status = handles(dev)
+    out = q.new_empty(q.shape)
+    nbytes = lib.vmk_prompt_workspace_bytes(S, Tq, Tk, Hq, Hkv, D) if Hkv else 0
+    if nbytes == 0:
+        raise _lib.VmkError(-2, "prompt: unsupported shape")
+    ws = scratch(nbytes, dev, stream)
+    rc = lib.vmk_prompt(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), _strides(q, k, v),
+                        out.data_ptr(), S, Tq, Tk, Hq, Hkv, D, 1 if causal else 0, 1 if dt == torch.bfloat16 else 0,
+                        *ws, status, stream)
     _lib.check(rc, "vmk_prompt")
     return _lib.finish(out, host, check, dev, "vmk_prompt")
 
@@ -108,16 +110,18 @@ def kernel_paged(q, k_pages, v_pages, page_table, cu_q, lens, causal=True, check
     if k_pages.device != dev or v_pages.device != dev or cu_q.device != dev:
         _same_device(dev, k_pages=k_pages, v_pages=v_pages, cu_q=cu_q)
     lib = _lib.lib()
-    with _lib.on_device(dev):
-        stream = _lib.raw_stream(dev)
-        out = q.new_empty(q.shape)
-        nbytes = lib.vmk_prompt_workspace_bytes(S, Tq, T * page_size, Hq, Hkv, D) if Hkv else 0
-        if nbytes == 0:
-            raise _lib.VmkError(-2, "prompt: unsupported shape")
-        ws = _lib.scratch(nbytes, dev, stream)
-        rc = lib.vmk_prompt_paged(_lib.ptr(q), _lib.ptr(k_pages), _lib.ptr(v_pages), _lib.ptr(page_table), pages, page_size,
-                                  T, _lib.ptr(cu_q), _lib.ptr(lens), _strides(q), _lib.ptr(out), S, Tq, Hq, Hkv, D,
-                                  1 if causal else 0, 1 if dt == torch.bfloat16 else 0, _lib.ptr(ws), ws.numel(),
-                                  _lib.ptr(_lib.status_word(dev)), stream)
+    if elsewhere(dev):
+        with torch.cuda.device(dev):
+            return kernel_paged(q, k_pages, v_pages, page_table, cu_q, lens, causal, check)
+    stream, status = handles(dev)
+    out = q.new_empty(q.shape)
+    nbytes = lib.vmk_prompt_workspace_bytes(S, Tq, T * page_size, Hq, Hkv, D) if Hkv else 0
+    if nbytes == 0:
+        raise _lib.VmkError(-2, "prompt: unsupported shape")
+    ws = scratch(nbytes, dev, stream)
+    rc = lib.vmk_prompt_paged(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), pages, page_size,
+                              T, cu_q.data_ptr(), lens.data_ptr(), _strides(q), out.data_ptr(), S, Tq, Hq, Hkv, D,
+                              1 if causal else 0, 1 if dt == torch.bfloat16 else 0, *ws,
+                              status, stream)
     _lib.check(rc, "vmk_prompt_paged")
     return _lib.finish(out, False, check, dev, "vmk_prompt_paged")
