@@ -303,3 +303,14 @@ def test_a_nan_key_in_one_share_reaches_every_row():
     inp["k"][3000, 0] = np.nan
     out = prompt_b200.kernel(**_dev(inp, torch.float16), check=True)
     assert torch.isnan(out[:, :2]).all() and torch.equal(out[:, 2:], clean[:, 2:])
+
+
+def test_sequences_that_overlap_are_reported_and_stay_inside_their_tensors():
+    """More tiles than the rows of q come to: a list of lengths that goes up and down, long enough for the planner."""
+    q = torch.randn(5000, 4, 128, device="cuda").half()
+    k = torch.randn(5000, 1, 128, device="cuda").half()
+    cu = torch.tensor([0, 5000] * 600 + [0], dtype=torch.int32, device="cuda")
+    out = prompt_b200.kernel(q, k, k, cu)
+    with pytest.raises(_lib.VmkDeviceStatusError) as e:
+        check_status(out.device)
+    assert e.value.status == 2 and out.shape == q.shape

@@ -56,6 +56,7 @@ constexpr int kPmPlanThreads = 1024;
 constexpr int kPmSplitMin = 4;                   // key blocks that a split is worth
 constexpr int kPmMaxSplit = 32;
 constexpr int kPmBins = 256;
+constexpr int kPmMaxItems = 1 << 20;             // tiles of a call: 16 million tokens at 16 heads a group, 268 million at one
 
 struct PromptItem {          // one 256-row tile of one sequence
   int tok0;                  // first query token (index into q)
@@ -160,11 +161,13 @@ __global__ void __launch_bounds__(kPmPlanThreads, 1) prompt_plan_kernel(const Pr
   bool bad = false;
   // Pass 0 counts the tiles of each cost, pass 1 places them, the costly ones first.
   for (int pass = 0; pass < 2; ++pass) {
+    int listed = 0;
     for (int base = 0; base < sq.S; base += kPmPlanThreads) {
       const int s = base + tid;
       int q0 = 0, nq = 0, k0 = 0, nk = 0;
       if (s < sq.S) bad |= prompt_seq(sq, s, q0, nq, k0, nk);
-      const int tiles = (nq + per - 1) / per;
+      // (sequences that overlap could come to more tiles than the list has room for: sums stay below 2^31 all the same)
+      const int tiles = min((nq + per - 1) / per, p.max_items + 1);
       int incl = tiles;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -192,7 +195,9 @@ __global__ void __launch_bounds__(kPmPlanThreads, 1) prompt_plan_kernel(const Pr
       s_nk[tid] = nk;
       if (tid == kPmPlanThreads - 1) s_start[kPmPlanThreads] = incl;
       __syncthreads();
-      const int total = s_start[kPmPlanThreads];
+      const int room = p.max_items - listed, total = min(s_start[kPmPlanThreads], room);
+      if (s_start[kPmPlanThreads] > room) bad = true;
+      listed += total;
       for (int i = tid; i < total; i += kPmPlanThreads) {
         int lo = 0, hi = kPmPlanThreads;        // the last sequence whose first tile is at or before i
         while (hi - lo > 1) {
@@ -206,8 +211,7 @@ __global__ void __launch_bounds__(kPmPlanThreads, 1) prompt_plan_kernel(const Pr
         if (pass == 0) {
           atomicAdd(&s_hist[bin], 1);
         } else {
-          const int at = atomicAdd(&s_hist[bin], 1);
-          if (at < p.max_items) p.items[at] = it;
+          p.items[atomicAdd(&s_hist[bin], 1)] = it;
         }
       }
     }
@@ -238,9 +242,8 @@ __global__ void __launch_bounds__(kPmPlanThreads, 1) prompt_plan_kernel(const Pr
     }
   }
   if (tid == 0) {
-    p.ctrl->n_items = min(s_total, p.max_items);
+    p.ctrl->n_items = s_total;
     p.ctrl->next = p.first_units;
-    if (s_total > p.max_items) bad = true;      // sequences that overlap: more rows than q has
   }
   if (bad) report(p.status, kStatusBadIndex);
 }
@@ -326,7 +329,7 @@ __device__ __forceinline__ void prompt_share(PromptUnit& u, int tpt, int nsplit,
   u.nb = max(0, min(nb, j1) - j0);
 }
 
-constexpr int kPmBars = 2 * kPmSlots + 2 * kPmSched + 2 + 2 + 2 + 2 + 2 + 2;
+constexpr int kPmBars = 2 * kPmSlots + 2 * kPmSched + 2 + 2 + 2 + 2 + 2 + 2 + 2;   // (an even number: what follows is 16-byte aligned)
 constexpr int kPmSmem = 2 * kPmTile + kPmSlots * kPmTile + kPmBars * 8 + kPmSched * (int)sizeof(PromptUnit) + 16 + 1024;
 static_assert(kPmSmem <= 232448, "shared memory of one CTA");
 
@@ -346,6 +349,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
   uint64_t* p_part = s_full + 2;                         // [tile] P of the first 96 keys in tensor memory (4 warps)
   uint64_t* p_full = p_part + 2;                         // [tile] all of P                    (4 warps)
   uint64_t* o_full = p_full + 2;                         // [tile] last P.V of a unit done     (MMA commit)
+  uint64_t* drain = o_full + 2;                          // every product done, after a timeout
   PromptUnit* units = reinterpret_cast<PromptUnit*>(sKV + kPmSlots * kPmTile + kPmBars * 8);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(units + kPmSched);
 
@@ -367,6 +371,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
       mbar_init(&p_full[t], 4);
       mbar_init(&o_full[t], 1);
     }
+    mbar_init(drain, 1);
     fence_mbar_init();
   }
   if (warp == 9) tmem_alloc(tmem_slot, kPmCols);
@@ -489,7 +494,6 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
           const CUtensorMap* tm = (i & 1) ? &p.tmV : &p.tmK;
           uint8_t* dst = sKV + s * kPmTile;
           const int kb = (un.j0 + (i >> 1)) * kPmBK;
-          //TR(4, i >> 1, i & 1)
           mbar_expect_tx(&full[s], kPmTile);
           if (p.page_table == nullptr) {
             tma_load_3d(dst, tm, 0, un.h, un.it.k0 + kb, &full[s]);
@@ -544,9 +548,11 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
                   idesc_qk, k > 0 ? 1u : 0u);
       pm_commit(lead, &s_full[t]);
     };
-    for (uint32_t n = 0; !timed_out; ++n) {
+    for (uint32_t n = 0;; ++n) {
       const int sl = n % kPmSched;
-      if (!mbar_wait(&sched_full[sl], (n / kPmSched) & 1)) { timed_out = true; break; }
+      if (!mbar_wait(&sched_full[sl], (n / kPmSched) & 1)) timed_out = true;
+      // a wait that ran out for one lane ends the unit for it, and here the loop for all
+      if (__any_sync(0xffffffffu, timed_out)) { timed_out = true; break; }
       const int h = __shfl_sync(0xffffffffu, units[sl].h, 0);
       const int nt0 = __shfl_sync(0xffffffffu, units[sl].na, 0), nt1 = __shfl_sync(0xffffffffu, units[sl].nb, 0);
       __syncwarp();
@@ -567,48 +573,42 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
         qk(t, ring % kPmSlots);
         if (nt == 1) pm_commit(lead, &q_empty[t]);
       }
-      if (timed_out) break;
-      pm_commit(lead, &empty[ring % kPmSlots]);
+      if (!timed_out) pm_commit(lead, &empty[ring % kPmSlots]);
       for (int j = 0; j < nblk && !timed_out; ++j) {
         const uint32_t iv = ring + 2 * j + 1, ik = iv + 1;
         wait_tile(iv);
-        //TR(3, j, 7)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const int nt = t == 0 ? nt0 : nt1;
           if (j >= nt || timed_out) continue;
           const uint32_t o = tmem_base + kPmColO + t * 128, a = tmem_base + kPmColS + t * 128;
           const uint32_t b = v_lo + (iv % kPmSlots) * (kPmTile >> 4);
-          //TR(2 + t, j, 0)
           if (!mbar_wait(&p_part[t], n_p[t] & 1)) { timed_out = true; continue; }
-          //TR(2 + t, j, 1)
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < 6; ++k) pm_mma_ts(lead, o, a + k * 8, b + k * (2048 >> 4), hi_v, idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
           if (!mbar_wait(&p_full[t], n_p[t]++ & 1)) { timed_out = true; continue; }
-          //TR(2 + t, j, 2)
           tc_fence_after();
 #pragma unroll
           for (int k = 6; k < 8; ++k) pm_mma_ts(lead, o, a + k * 8, b + k * (2048 >> 4), hi_v, idesc_pv, 1u);
-          //TR(2 + t, j, 3)
           if (j + 1 == nt) {
             pm_commit(lead, &o_full[t]);
           } else {
             wait_tile(ik);
             if (timed_out) continue;
-            //TR(4, j, 2 + t)
             qk(t, ik % kPmSlots);
-            //TR(2 + t, j, 4)
             if (j + 2 == nt) pm_commit(lead, &q_empty[t]);
           }
         }
         if (timed_out) break;
-        //TR(3, j, 5)
         pm_commit(lead, &empty[iv % kPmSlots]);
         if (j + 1 < nblk) pm_commit(lead, &empty[ik % kPmSlots]);
-        //TR(3, j, 6)
       }
       ring += 2 * nblk;
+    }
+    if (timed_out) {                                       // the products in flight end before tensor memory is freed
+      pm_commit(lead, drain);
+      mbar_wait(drain, 0);
     }
   } else if (warp == 10) {
     // ------------------------------------------------------------------------------ rows outside every sequence
@@ -649,7 +649,6 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < mine; ++j) {
         if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], n_s++ & 1))) { timed_out = true; break; }
-        //TR(t, j, 0)
         tc_fence_after();
         const int kb = (j0 + j) * kPmBK;
         uint32_t sv[128];
@@ -658,7 +657,6 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
         tmem_ld32(tS + 64, *reinterpret_cast<uint32_t(*)[32]>(sv + 64));
         tmem_ld32(tS + 96, *reinterpret_cast<uint32_t(*)[32]>(sv + 96));
         tmem_ld_wait();
-        //TR(t, j, 1)
         const bool edge = kb + kPmBK > vis_all;
         if (edge) {
           // a block that the mask or the end of the keys cuts: hidden scores become -inf whatever they were
@@ -718,7 +716,6 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
           sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
           chunk(0, mu, sum);
         }
-        //TR(t, j, 2)
         if (kb + kPmBK > it.nk && (t == 0 || j >= na)) {
           // rows of V past the sequence's end are cleared by the tile whose product comes first
           const uint32_t iv = ring + 2 * j + 1;
@@ -743,12 +740,10 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
             if (lane == 0) mbar_arrive(&p_part[t]);
           }
         }
-        //TR(t, j, 3)
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
-        //TR(t, j, 4)
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       }
       if (timed_out) break;
@@ -855,7 +850,7 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptParams p)
 static int prompt_tiles_bound(int Tq, int S, int tpt) {
   // ceil(n / per) <= (n - 1) / per + 1 for every sequence that is not empty
   const long long s = S < Tq ? S : Tq, n = ((long long)Tq - s) / (2 * tpt) + s;
-  return n > 0x7fffffffll / 64 ? -1 : (int)n;
+  return n > kPmMaxItems ? -1 : (int)n;
 }
 
 // How a call is cut.  Up to one unit per SM, every CTA finds its unit itself, and where that leaves half of the SMs or more
