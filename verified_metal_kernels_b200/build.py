@@ -13,6 +13,10 @@ NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", 
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
 
 
+CALLS_SRC = os.path.join(CSRC, "torch_calls.cpp")
+CALLS_LIB = os.path.join(HERE, "_vmk_torch.so")
+
+
 def sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.cu")))
 
@@ -56,6 +60,54 @@ def build(force=False, verbose=False):
     return LIB
 
 
+def calls_fingerprint():
+    """Hash of what goes into _vmk_torch.so: its source, the C header, torch's and Python's versions."""
+    import torch
+    h = hashlib.sha256(f"{torch.__version__} {sys.version}".encode())
+    for d in (CALLS_SRC, os.path.join(HERE, "..", "include", "vmk_b200.h")):
+        with open(d, "rb") as f:
+            h.update(f.read())
+    return h.hexdigest()
+
+
+def build_calls(force=False):
+    """Compile torch_calls.cpp (the kernel modules' ordinary calls, torch tensors to the C entry points) with g++ against
+    torch's headers, in-tree.  Returns the path.  Locked and published like the library."""
+    import sysconfig
+
+    import torch
+    stamp = calls_fingerprint()
+
+    def fresh():
+        if force or not os.path.exists(CALLS_LIB) or not os.path.exists(CALLS_LIB + ".stamp"):
+            return False
+        with open(CALLS_LIB + ".stamp") as f:
+            return f.read().strip() == stamp
+
+    if fresh():
+        return CALLS_LIB
+    with open(os.path.join(HERE, ".build.lock"), "w") as lock:
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        try:
+            if not fresh():
+                root = os.path.dirname(torch.__file__)
+                tmp = CALLS_LIB + ".tmp.%d" % os.getpid()
+                cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+                       "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch.compiled_with_cxx11_abi(), "-I", sysconfig.get_paths()["include"]]
+                for d in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                          os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")):
+                    cmd += ["-isystem", d]
+                cmd += [CALLS_SRC, "-o", tmp, "-L", os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+                subprocess.check_call(cmd)
+                os.replace(tmp, CALLS_LIB)
+                with open(CALLS_LIB + ".stamp.tmp", "w") as f:
+                    f.write(stamp + "\n")
+                os.replace(CALLS_LIB + ".stamp.tmp", CALLS_LIB + ".stamp")
+        finally:
+            fcntl.flock(lock, fcntl.LOCK_UN)
+    return CALLS_LIB
+
+
 def _build_locked(verbose):
     nvcc = os.environ.get("NVCC", "nvcc")
     extra = os.environ.get("VMK_EXTRA_NVCC_FLAGS", "").split()      # e.g. -DVMK_TC_TIMING for device-side phase timers
@@ -85,3 +137,4 @@ def _build_locked(verbose):
 
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="-v" in sys.argv))
+    print(build_calls(force="--force" in sys.argv))

@@ -1,7 +1,15 @@
 """Argument checks shared by the kernel modules."""
+import ctypes
+import importlib.util
+import os
+
 import torch
 
 from .. import _lib
+
+_ENTRIES = ("vmk_prompt_workspace_bytes", "vmk_prompt", "vmk_prompt_paged", "vmk_accept", "vmk_pages_workspace_bytes",
+            "vmk_pages_reserve", "vmk_pages_append", "vmk_pages_fork", "vmk_pages_compact", "vmk_pages_free", "vmk_pages_copy")
+_calls = None
 
 
 def need(t, name, dtype, shape=None, dims=None):
@@ -46,9 +54,28 @@ def elsewhere(dev):
     return torch._C._cuda_getDevice() != dev.index
 
 
+def calls():
+    """The compiled form of the modules' ordinary calls (csrc/torch_calls.cpp), loaded on first use.  Its functions return
+    None, having done nothing, for every call that is not ordinary."""
+    global _calls
+    if _calls is None:
+        path = os.path.join(_lib.HERE, "_vmk_torch.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing: build it with `python -m verified_metal_kernels_b200.build`")
+        lib = _lib.lib()
+        spec = importlib.util.spec_from_file_location("_vmk_torch", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.init(*[ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _ENTRIES])
+        _calls = module
+    return _calls
+
+
 def handles(dev):
     """Torch's current stream on `dev` as an integer (no Stream object is built) and the address of the device's status word."""
-    return torch._C._cuda_getCurrentRawStream(dev.index), _lib.status_word(dev).data_ptr()
+    status = _lib.status_word(dev).data_ptr()
+    calls().set_status(dev.index, status)
+    return torch._C._cuda_getCurrentRawStream(dev.index), status
 
 
 def scratch(nbytes, dev, stream):

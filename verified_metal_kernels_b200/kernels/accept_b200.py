@@ -5,7 +5,7 @@ it is the step after `spec`, once the target's probabilities of every draft row 
 import torch
 
 from .. import _lib
-from ._common import elsewhere, handles, need, need_on, stage_in
+from ._common import calls, elsewhere, handles, need, need_on, stage_in
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
@@ -25,6 +25,10 @@ def kernel(target_probs, tokens, bits, u, draft_probs=None, check=False):
     that are NaN, infinite or negative count as 0; a row of nothing but those gives next_token -1.  A draft token outside
     [0, V) is refused (and reported in the device status word).  Host tensors are copied in and the results returned on
     the host."""
+    if not check:
+        out = calls().accept(target_probs, tokens, bits, u, draft_probs)
+        if out is not None:
+            return out
     (target_probs, tokens, bits, u, draft_probs), host = stage_in([target_probs, tokens, bits, u, draft_probs])
     if not isinstance(target_probs, torch.Tensor) or target_probs.dtype not in DTYPES:
         raise TypeError("target_probs: expected a float32, float16 or bfloat16 tensor")

@@ -16,7 +16,7 @@ import struct
 import torch
 
 from .. import _lib
-from ._common import elsewhere, handles, need, need_on, scratch
+from ._common import calls, elsewhere, handles, need, need_on, scratch
 
 
 def _state(page_table, lens, refs):
@@ -78,6 +78,10 @@ def reserve(page_table, lens, refs, extra, page_size, check=False):
     """Row r grows by extra[r] (>= 0) positions: it gets the pages that it lacks, and lens[r] += extra[r].  A row gets all its
     pages or, where what it and the rows before it need exceeds the free pages (or its table is too short), none, and
     stays as it is.  Returns granted (R,) int32, 1 or 0."""
+    if not check:
+        granted = calls().reserve(page_table, lens, refs, extra, page_size)
+        if granted is not None:
+            return granted
     R, T, dev = _state(page_table, lens, refs)
     need_on(extra, "extra", torch.int32, (R,), dev)
     lib = _lib.lib()
@@ -98,6 +102,8 @@ def append(k, v, k_pages, v_pages, page_table, cu, lens, check=False):
     and tokens [cu[s], cu[s+1]) of row s become its last positions: lens[s] counts them already (reserve before append).
     k_pages, v_pages (pages,heads,page_size,width), or (pages,page_size,width) for one head; k and v may differ in
     heads and width (dsa: latent rows and index keys).  Tokens outside [cu[0], cu[-1]) are not written."""
+    if not check and calls().append(k, v, k_pages, v_pages, page_table, cu, lens):
+        return
     R, T, dev = _state(page_table, lens, None)
     need(cu, "cu", torch.int32, dims=1)
     S = cu.shape[0] - 1
@@ -138,6 +144,8 @@ def fork(pools, page_table, lens, refs, parents, children, check=False):
     pages are shared, the used rows of a last page that is not full are copied into a page of its own, in every pool.
     parents[f] < 0: an entry that does nothing.  Refused (and reported): a child that is not empty, out of range, or
     named a second time; entries for which no free page is left."""
+    if not check and calls().fork(pools, page_table, lens, refs, parents, children):
+        return
     R, T, dev = _state(page_table, lens, refs)
     desc, pages, page_size = _pools(pools, dev)
     _need_refs(refs, pages)
@@ -160,6 +168,8 @@ def compact(pools, page_table, lens, refs, path, count, check=False):
     """After kd drafts at the end of each row were verified: the accepted ones, path (R,kd) int32 and count (R,) int32 as
     accept_b200.kernel gives them, close up behind the positions before the drafts, lens[r] becomes lens[r] - kd +
     count[r], and pages behind that are given back.  count[r] < 0: the row stays as it is."""
+    if not check and calls().compact(pools, page_table, lens, refs, path, count):
+        return
     R, T, dev = _state(page_table, lens, refs)
     desc, pages, page_size = _pools(pools, dev)
     _need_refs(refs, pages)
@@ -180,6 +190,8 @@ def compact(pools, page_table, lens, refs, path, count, check=False):
 def free(page_table, lens, refs, keep, page_size, check=False):
     """Row r keeps its first keep[r] (>= 0) positions; the pages behind them are given back (a page that other rows share
     stays theirs), and their slots become -1.  keep[r] = 0 frees the row, keep[r] >= lens[r] leaves it as it is."""
+    if not check and calls().free(page_table, lens, refs, keep, page_size):
+        return
     R, T, dev = _state(page_table, lens, refs)
     need_on(keep, "keep", torch.int32, (R,), dev)
     lib = _lib.lib()
@@ -195,6 +207,8 @@ def free(page_table, lens, refs, keep, page_size, check=False):
 def copy(pools, src, dst, check=False):
     """Page src[i] -> page dst[i] in every pool and layer; src, dst (n,) int32.  No page may be both in src and in dst, or
     twice in dst."""
+    if not check and calls().copy(pools, src, dst):
+        return
     if isinstance(pools, torch.Tensor) or not pools or not isinstance(pools[0], torch.Tensor):
         raise ValueError("pools: expected a list of 1 to 8 tensors")
     dev = pools[0].device

@@ -8,7 +8,7 @@ import struct
 import torch
 
 from .. import _lib
-from ._common import elsewhere, handles, need, need_on, scratch, stage_in
+from ._common import calls, elsewhere, handles, need, need_on, scratch, stage_in
 
 
 def _rows(t, name, dtype):
@@ -64,6 +64,10 @@ def kernel(q, k, v, cu_q, cu_k=None, causal=True, check=False):
     causal=False all of them.  A query that sees no key gets zeros, and so do rows outside [cu_q[0], cu_q[-1]).
     q, k and v may be views (see the strides that _rows allows).  Host tensors are copied in and the result returned
     on the host (with the device status word checked; device-resident calls check it only with check=True)."""
+    if not check:
+        out = calls().prompt(q, k, v, cu_q, cu_k, causal)
+        if out is not None:
+            return out
     (q, k, v, cu_q, cu_k), host = stage_in([q, k, v, cu_q, cu_k])
     dt, Tq, Hq, D, S = _common(q, cu_q)
     _rows(k, "k", dt)
@@ -95,6 +99,10 @@ def kernel(q, k, v, cu_q, cu_k=None, causal=True, check=False):
 def kernel_paged(q, k_pages, v_pages, page_table, cu_q, lens, causal=True, check=False):
     """The same over a paged cache: k_pages / v_pages (pages,Hkv,page_size,128), page_table (S,T) int32, lens (S,)
     int32 the keys of each sequence, its new tokens (already appended) included; page_size a multiple of 64."""
+    if not check:
+        out = calls().prompt_paged(q, k_pages, v_pages, page_table, cu_q, lens, causal)
+        if out is not None:
+            return out
     dt, Tq, Hq, D, S = _common(q, cu_q)
     need(k_pages, "k_pages", dt, dims=4)
     pages, Hkv, page_size = k_pages.shape[0], k_pages.shape[1], k_pages.shape[2]
