@@ -47,6 +47,7 @@ constexpr int kPmD = 128;
 constexpr int kPmHalf = 128 * 128;               // [128 rows][128 B] swizzled: one 64-wide half of the head dim
 constexpr int kPmTile = 2 * kPmHalf;             // 32 KiB: a Q, K or V tile
 constexpr int kPmSlots = 5;
+constexpr int kPmTwinSlots = 6;                  // where both tiles read one Q tile (prompt_twin), the other's place is a slot
 constexpr int kPmSched = 2;
 constexpr int kPmThreads = 384;                // 12 warps x 168 registers; after set-up 2 x 128 threads hold 216, 128 hold 72
 constexpr int kPmCols = 512;
@@ -307,6 +308,7 @@ struct PromptUnit {          // what warp 8 hands to the others
   PromptItem it;
   int h;                     // kv head; -1: no more units
   int j0, na, nb;            // first key block of this CTA's share, and how many of it tiles A and B have to see
+  int twin;                  // both tiles hold the same rows, and take the blocks j0, j0 + 2, ... and j0 + 1, j0 + 3, ...
 };
 
 // Key blocks that 128-row tile t of an item has to see, and how many tokens it holds.
@@ -316,6 +318,12 @@ __device__ __forceinline__ int tile_blocks(const PromptItem& it, int t, int tpt)
   const int seen = min(it.nk, max(0, it.vis0 + tok));
   return (seen + kPmBK - 1) / kPmBK;
 }
+
+// Shared units of one 128-row tile: tile B takes every other block of the same rows (one tile alone leaves the tensor pipe
+// idle during its softmax and the other way round), and the merge joins the two like shares of their own.  Both read one Q
+// tile; the other's place is a sixth slot of the ring.  (17 tokens over 60001 keys: 62.6 us with one tile, 57.0 with two; the
+// keys alone take 38 us to read.  Asking for later blocks into L2 ahead of the ring made it 64 to 71.)
+__device__ __forceinline__ bool prompt_twin(const PromptItem& it, int tpt, int nsplit) { return nsplit > 1 && it.ntok <= tpt; }
 
 // This CTA's share of a unit's key blocks: all of them, or part `sp` of `ns` equal ones of at least kPmSplitMin blocks.
 __device__ __forceinline__ int prompt_parts(int nblk, int nsplit) { return max(1, min(nsplit, nblk / kPmSplitMin)); }
@@ -327,21 +335,28 @@ __device__ __forceinline__ void prompt_share(PromptUnit& u, int tpt, int nsplit,
   u.j0 = j0;
   u.na = max(0, min(na, j1) - j0);
   u.nb = max(0, min(nb, j1) - j0);
+  u.twin = prompt_twin(u.it, tpt, nsplit);
+  if (u.twin) {
+    u.nb = u.na / 2;
+    u.na -= u.nb;
+  }
 }
 
-constexpr int kPmBars = 2 * kPmSlots + 2 * kPmSched + 2 + 2 + 2 + 2 + 2 + 2 + 2;   // (an even number: what follows is 16-byte aligned)
+constexpr int kPmBars = 2 * kPmTwinSlots + 2 * kPmSched + 2 + 2 + 2 + 2 + 2 + 2 + 2;   // (an even number: what follows is 16-byte aligned)
 constexpr int kPmSmem = 2 * kPmTile + kPmSlots * kPmTile + kPmBars * 8 + kPmSched * (int)sizeof(PromptUnit) + 16 + 1024;
 static_assert(kPmSmem <= 232448, "shared memory of one CTA");
 
-template <bool BF>
+// SPLIT: CTAs share units' keys and emit partials (always direct: one unit each).  An instance of its own, so that the
+// loops of the others hold nothing of it.
+template <bool BF, bool SPLIT>
 __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_constant__ PromptParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                                    // [2 tiles][32 KiB]
   uint8_t* sKV = sQ + 2 * kPmTile;                       // [slots][32 KiB]
   uint64_t* full = reinterpret_cast<uint64_t*>(sKV + kPmSlots * kPmTile);   // K or V tile landed (TMA bytes)
-  uint64_t* empty = full + kPmSlots;                     // consumed by both tiles' products   (MMA commit)
-  uint64_t* sched_full = empty + kPmSlots;               // unit written                       (warp 8)
+  uint64_t* empty = full + kPmTwinSlots;                 // consumed by both tiles' products   (MMA commit)
+  uint64_t* sched_full = empty + kPmTwinSlots;           // unit written                       (warp 8)
   uint64_t* sched_empty = sched_full + kPmSched;         // unit read by everybody             (9 warps)
   uint64_t* q_full = sched_empty + kPmSched;             // [tile] Q tile landed               (TMA bytes)
   uint64_t* q_empty = q_full + 2;                        // [tile] last Q.K^T of a unit done   (MMA commit)
@@ -355,7 +370,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int s = 0; s < kPmSlots; ++s) {
+    for (int s = 0; s < kPmTwinSlots; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -393,7 +408,8 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
     if (tid == 0) units[0].h = -1;
     int before = 0;
     bool bad = false;
-    for (int base = 0; base < p.seqs.S && before <= want; base += kPmThreads) {
+    // (CTA 0 looks at all of them, so that a list that does not ascend is reported wherever it does not)
+    for (int base = 0; base < p.seqs.S && (before <= want || blockIdx.x == 0); base += kPmThreads) {
       int q0 = 0, nq = 0, k0 = 0, nk = 0;
       if (base + tid < p.seqs.S) bad |= prompt_seq(p.seqs, base + tid, q0, nq, k0, nk);
       const int tiles = (nq + 2 * p.tpt - 1) / (2 * p.tpt);
@@ -441,7 +457,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
       const uint32_t q_bytes = (uint32_t)(p.tpt * p.G) * 128u * 2u;
       const int pool_pages = p.page_groups / p.Hkv;
       int u = blockIdx.x;
-      uint32_t ring = 0, issued_q[2] = {0, 0};
+      uint32_t ring = 0, issued_q[2] = {0, 0}, slots = kPmSlots;
       for (uint32_t n = 0;; ++n) {
         const int sl = n % kPmSched;
         if (n >= kPmSched && !mbar_wait(&sched_empty[sl], (n / kPmSched - 1) & 1)) { timed_out = true; break; }
@@ -457,7 +473,10 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
         units[sl] = un;
         mbar_arrive(&sched_full[sl]);
         if (un.h < 0) break;
-        const int nt0 = un.na, nt1 = un.nb, nblk = max(nt0, nt1);
+        const bool twin = SPLIT && un.twin;
+        if (twin) slots = kPmTwinSlots;
+        uint8_t* ring0 = twin ? sKV - kPmTile : sKV;
+        const int nt0 = un.na, nt1 = un.nb, nblk = twin ? nt0 + nt1 : max(nt0, nt1);
         // Paged keys: a block is two 64-key boxes, each inside one page; page ids are read one block ahead, and positions
         // are kept by counting (a division for each took this thread longer than a block).
         int pg = 0, off = 0, id[2] = {-1, -1}, next_id[2] = {-1, -1}, y[2] = {0, 0}, next_y[2] = {0, 0};
@@ -489,10 +508,10 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
             }
             if (i + 2 < 2 * nblk) look();
           }
-          const int s = ring % kPmSlots;
-          if (ring >= kPmSlots && !mbar_wait(&empty[s], (ring / kPmSlots - 1) & 1)) { timed_out = true; break; }
+          const int s = ring % slots;
+          if (ring >= slots && !mbar_wait(&empty[s], (ring / slots - 1) & 1)) { timed_out = true; break; }
           const CUtensorMap* tm = (i & 1) ? &p.tmV : &p.tmK;
-          uint8_t* dst = sKV + s * kPmTile;
+          uint8_t* dst = ring0 + s * kPmTile;
           const int kb = (un.j0 + (i >> 1)) * kPmBK;
           mbar_expect_tx(&full[s], kPmTile);
           if (p.page_table == nullptr) {
@@ -509,7 +528,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
           if (i == 0) {
             // the queries behind the first keys: the slot of K_0 is free earlier than the Q tiles of the unit before
             for (int t = 0; t < 2 && !timed_out; ++t) {
-              if ((t == 0 ? nt0 : nt1) == 0) continue;
+              if ((t == 0 ? nt0 : twin ? 0 : nt1) == 0) continue;
               if (issued_q[t] > 0 && !mbar_wait(&q_empty[t], (issued_q[t] - 1) & 1)) { timed_out = true; break; }
               ++issued_q[t];
               mbar_expect_tx(&q_full[t], q_bytes);
@@ -523,7 +542,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
         if (!p.direct) u = atomicAdd(&p.ctrl->next, 1);
       }
       // no load outlives the CTA: the newest tile of every slot has landed before this warp goes to the exit
-      for (uint32_t i = ring > kPmSlots ? ring - kPmSlots : 0; i < ring; ++i) mbar_wait(&full[i % kPmSlots], (i / kPmSlots) & 1);
+      for (uint32_t i = ring > slots ? ring - slots : 0; i < ring; ++i) mbar_wait(&full[i % slots], (i / slots) & 1);
       for (int t = 0; t < 2; ++t)
         if (issued_q[t] > 0) mbar_wait(&q_full[t], (issued_q[t] - 1) & 1);
     }
@@ -555,6 +574,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
       if (__any_sync(0xffffffffu, timed_out)) { timed_out = true; break; }
       const int h = __shfl_sync(0xffffffffu, units[sl].h, 0);
       const int nt0 = __shfl_sync(0xffffffffu, units[sl].na, 0), nt1 = __shfl_sync(0xffffffffu, units[sl].nb, 0);
+      const bool twin = SPLIT && __shfl_sync(0xffffffffu, units[sl].twin, 0) != 0;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sched_empty[sl]);
       if (h < 0) break;
@@ -563,6 +583,61 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
       auto wait_tile = [&](uint32_t i) {
         if (!mbar_wait(&full[i % kPmSlots], (i / kPmSlots) & 1)) timed_out = true;
       };
+      if constexpr (SPLIT) {
+        if (twin) {                                        // block j belongs to tile j & 1 alone
+          const int all = nt0 + nt1;
+          const uint32_t k6 = k_lo - (kPmTile >> 4), v6 = v_lo - (kPmTile >> 4);       // six slots, the second Q tile's place among them
+          auto landed = [&](uint32_t i) {
+            if (!mbar_wait(&full[i % kPmTwinSlots], (i / kPmTwinSlots) & 1)) timed_out = true;
+          };
+          auto qk_twin = [&](int t, uint32_t slot) {
+            const uint32_t d = tmem_base + kPmColS + t * 128, b = k6 + slot * (kPmTile >> 4);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              pm_mma_ss(lead, d, q_lo + (k >> 2) * (kPmHalf >> 4) + (k & 3) * 2, hi_k, b + (k >> 2) * (kPmHalf >> 4) + (k & 3) * 2, hi_k,
+                        idesc_qk, k > 0 ? 1u : 0u);
+            pm_commit(lead, &s_full[t]);
+            pm_commit(lead, &empty[slot]);
+          };
+          if (!mbar_wait(&q_full[0], 0)) timed_out = true;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (t >= all || timed_out) continue;
+            landed(2 * t);
+            if (timed_out) continue;
+            tc_fence_after();
+            qk_twin(t, 2 * t);
+          }
+          for (int j0 = 0; j0 < all && !timed_out; j0 += 2) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const int j = j0 + t;
+              if (j >= all || timed_out) continue;
+              const uint32_t iv = 2 * j + 1, ik = iv + 3;
+              landed(iv);
+              const uint32_t o = tmem_base + kPmColO + t * 128, a = tmem_base + kPmColS + t * 128;
+              const uint32_t b = v6 + (iv % kPmTwinSlots) * (kPmTile >> 4);
+              if (timed_out || !mbar_wait(&p_part[t], n_p[t] & 1)) { timed_out = true; continue; }
+              tc_fence_after();
+#pragma unroll
+              for (int k = 0; k < 6; ++k) pm_mma_ts(lead, o, a + k * 8, b + k * (2048 >> 4), hi_v, idesc_pv, (j0 > 0 || k > 0) ? 1u : 0u);
+              if (!mbar_wait(&p_full[t], n_p[t]++ & 1)) { timed_out = true; continue; }
+              tc_fence_after();
+#pragma unroll
+              for (int k = 6; k < 8; ++k) pm_mma_ts(lead, o, a + k * 8, b + k * (2048 >> 4), hi_v, idesc_pv, 1u);
+              if (j + 2 >= all) {
+                pm_commit(lead, &o_full[t]);
+              } else {
+                landed(ik);
+                if (timed_out) continue;
+                qk_twin(t, ik % kPmTwinSlots);
+              }
+              pm_commit(lead, &empty[iv % kPmTwinSlots]);
+            }
+          }
+          continue;                                        // (a CTA has one such unit)
+        }
+      }
       wait_tile(ring);                                     // K_0
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -636,21 +711,23 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
       if (!__all_sync(0xffffffffu, mbar_wait(&sched_full[sl], (n / kPmSched) & 1))) { timed_out = true; break; }
       const PromptItem it = units[sl].it;
       const int h = units[sl].h, j0 = units[sl].j0, na = units[sl].na, nb = units[sl].nb;
+      const bool twin = SPLIT && units[sl].twin;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sched_empty[sl]);
       if (h < 0) break;
-      const int nblk = max(na, nb), mine = t == 0 ? na : nb;
-      const int tk = t * p.tpt + tok;                     // token of the row inside the item
+      const int nblk = twin ? na + nb : max(na, nb), mine = t == 0 ? na : nb;
+      const int tile0 = twin ? 0 : t * p.tpt;             // the tile's first token inside the item
+      const int tk = tile0 + tok;                         // that of the row
       const bool valid = tok < p.tpt && tk < it.ntok;
       const int vis = valid ? min(it.nk, max(0, it.vis0 + tk + 1)) : 0;
       // keys that every row of this tile sees (its first token's)
-      const int vis_all = min(it.nk, max(0, it.vis0 + t * p.tpt + 1));
+      const int vis_all = min(it.nk, max(0, it.vis0 + tile0 + 1));
 
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < mine; ++j) {
         if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], n_s++ & 1))) { timed_out = true; break; }
         tc_fence_after();
-        const int kb = (j0 + j) * kPmBK;
+        const int blk = twin ? 2 * j + t : j, kb = (j0 + blk) * kPmBK;
         uint32_t sv[128];
         tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(sv));
         tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
@@ -716,11 +793,11 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
           sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
           chunk(0, mu, sum);
         }
-        if (kb + kPmBK > it.nk && (t == 0 || j >= na)) {
+        if (kb + kPmBK > it.nk && (twin || t == 0 || j >= na)) {
           // rows of V past the sequence's end are cleared by the tile whose product comes first
-          const uint32_t iv = ring + 2 * j + 1;
-          if (!__all_sync(0xffffffffu, mbar_wait(&full[iv % kPmSlots], (iv / kPmSlots) & 1))) { timed_out = true; break; }
-          uint8_t* v = sKV + (iv % kPmSlots) * kPmTile;
+          const uint32_t iv = ring + 2 * blk + 1, slots = twin ? kPmTwinSlots : kPmSlots;
+          if (!__all_sync(0xffffffffu, mbar_wait(&full[iv % slots], (iv / slots) & 1))) { timed_out = true; break; }
+          uint8_t* v = sKV + (iv % slots) * kPmTile - (twin ? kPmTile : 0);
           const int r0 = it.nk - kb;
           for (int e = row; e < (kPmBK - r0) * 16; e += 128) {
             const int r = r0 + (e >> 4), c = e & 15;
@@ -754,7 +831,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
         if (!__all_sync(0xffffffffu, mbar_wait(&o_full[t], n_o++ & 1))) { timed_out = true; break; }
         tc_fence_after();
       }
-      if (p.nsplit > 1) {
+      if constexpr (SPLIT) {
         // a share of the keys: the row's maximum, sum and unnormalised output, for the merge
         const size_t at = (size_t)blockIdx.x * 256 + t * 128 + row;
         if (valid) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mine > 0 ? m : -INFINITY, l);
@@ -820,24 +897,49 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptParams p)
   const int t = r >> 7, tok = (r & 127) / p.G, g = (r & 127) - tok * p.G, tk = t * p.tpt + tok;
   if (tok >= p.tpt || tk >= it.ntok) return;
   const int parts = prompt_parts(max(tile_blocks(it, 0, p.tpt), tile_blocks(it, 1, p.tpt)), p.nsplit);
+  const int tiles = prompt_twin(it, p.tpt, p.nsplit) ? 2 : 1;     // of a share that hold this row
   const size_t at0 = (size_t)u * p.nsplit * 256 + r;
-  float2 ml = make_float2(-INFINITY, 0.f);
-  if (lane < parts) ml = *reinterpret_cast<const float2*>(p.part_ml + (at0 + (size_t)lane * 256) * 2);
-  // the maximum leaves a NaN share out of m, but its l is NaN and reaches the sum
-  const float m = warp_max(ml.x);
-  const float w = ml.x == -INFINITY ? 0.f : pm_exp2(ml.x - m);
-  const float l = warp_sum(ml.x == -INFINITY && ml.y == 0.f ? 0.f : w * ml.y);
+  float2 ml[2];
+  float m = -INFINITY;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    ml[s] = make_float2(-INFINITY, 0.f);
+    if (lane < parts && s < tiles) ml[s] = *reinterpret_cast<const float2*>(p.part_ml + (at0 + (size_t)lane * 256 + s * 128) * 2);
+    // the maximum leaves a NaN share out of m, but its l is NaN and reaches the sum
+    m = fmaxf(m, ml[s].x);
+  }
+  m = warp_max(m);
+  float w[2], l = 0.f;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    w[s] = ml[s].x == -INFINITY ? 0.f : pm_exp2(ml[s].x - m);
+    l += ml[s].x == -INFINITY && ml[s].y == 0.f ? 0.f : w[s] * ml[s].y;
+  }
+  l = warp_sum(l);
   const float scale = l > 0.f || l != l ? 1.f / l : 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
-    const float wi = __shfl_sync(0xffffffffu, w, i);
-    if (wi == 0.f) continue;                             // a share that this row sees nothing of may not have been written
-    const float4 v = *reinterpret_cast<const float4*>(p.part_o + (at0 + (size_t)i * 256) * kPmD + lane * 4);
-    o.x += wi * v.x;
-    o.y += wi * v.y;
-    o.z += wi * v.z;
-    o.w += wi * v.w;
+  for (int i = 0; i < parts; i += 8) {                   // (loads under predicates: sixteen are in flight)
+    float4 v[8][2];
+    float wi[8][2];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        wi[k][s] = __shfl_sync(0xffffffffu, w[s], (i + k) & 31);
+        if (i + k >= parts) wi[k][s] = 0.f;
+        v[k][s] = make_float4(0.f, 0.f, 0.f, 0.f);
+        // a share that this row sees nothing of may not have been written
+        if (wi[k][s] != 0.f) v[k][s] = *reinterpret_cast<const float4*>(p.part_o + (at0 + (size_t)(i + k) * 256 + s * 128) * kPmD + lane * 4);
+      }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        o.x += wi[k][s] * v[k][s].x;
+        o.y += wi[k][s] * v[k][s].y;
+        o.z += wi[k][s] * v[k][s].z;
+        o.w += wi[k][s] * v[k][s].w;
+      }
   }
   uint2 out = make_uint2(0u, 0u);
   if (scale != 0.f) out = make_uint2(pack2(o.x * scale, o.y * scale, p.bf16), pack2(o.z * scale, o.w * scale, p.bf16));
@@ -932,8 +1034,9 @@ static int prompt_impl(const void* q, const void* k, const void* v, const int32_
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return VMK_E_LAUNCH;
   if (dev >= 64 || !(configured.load() >> dev & 1)) {
-    cudaError_t e = cudaFuncSetAttribute(prompt_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPmSmem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(prompt_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPmSmem);
+    cudaError_t e = cudaSuccess;
+    for (auto kernel : {prompt_kernel<false, false>, prompt_kernel<false, true>, prompt_kernel<true, false>, prompt_kernel<true, true>})
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPmSmem);
     if (e != cudaSuccess) return check_launch(e);
     if (dev < 64) configured.fetch_or(1ull << dev);
   }
@@ -984,7 +1087,9 @@ static int prompt_impl(const void* q, const void* k, const void* v, const int32_
   cfg.gridDim = dim3(pl.grid);
   cfg.blockDim = dim3(kPmThreads);
   cfg.dynamicSmemBytes = kPmSmem;
-  rc = check_launch(bf16 ? cudaLaunchKernelEx(&cfg, prompt_kernel<true>, p) : cudaLaunchKernelEx(&cfg, prompt_kernel<false>, p));
+  const auto kernel = pl.nsplit > 1 ? (bf16 ? prompt_kernel<true, true> : prompt_kernel<false, true>)
+                                    : (bf16 ? prompt_kernel<true, false> : prompt_kernel<false, false>);
+  rc = check_launch(cudaLaunchKernelEx(&cfg, kernel, p));
   if (rc != VMK_OK || pl.nsplit == 1) return rc;
   cfg.gridDim = dim3(pl.grid / pl.nsplit * 32);
   cfg.blockDim = dim3(256);
