@@ -314,3 +314,26 @@ def test_sequences_that_overlap_are_reported_and_stay_inside_their_tensors():
     with pytest.raises(_lib.VmkDeviceStatusError) as e:
         check_status(out.device)
     assert e.value.status == 2 and out.shape == q.shape
+
+
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (7, 1), (16, 1), (4, 4)])
+def test_sequences_of_one_and_of_two_tiles_share_in_one_call(hq, hkv):
+    """A sequence whose rows fit one 128-row tile has them in both, which take its blocks in turn; odd and even numbers of
+    blocks to a share, shares of one block, NaN behind the last key."""
+    tpt = 128 // (hq // hkv)
+    for seqs in ([(tpt + 3, 2000), (tpt, 2000)], [(1, 513), (2 * tpt, 1153), (tpt - 1, 640)], [(3, 4096 + 65)], [(5, 1), (2, 1037)]):
+        inp = _inputs(seqs, hq, hkv, torch.float16, seed=101, pad_q=3, pad_k=70, fill=np.nan)
+        out = prompt_b200.kernel(**_dev(inp, torch.float16), check=True)
+        n = sum(a for a, _ in seqs)
+        assert (out[n:] == 0).all()
+        inp = {**inp, "q": inp["q"][:n], "k": inp["k"][:sum(m for _, m in seqs)], "v": inp["v"][:sum(m for _, m in seqs)]}
+        _check(out[:n], inp, seqs, torch.float16)
+
+
+def test_a_short_list_that_does_not_ascend_is_reported():
+    q = torch.randn(40, 8, 128, device="cuda").half()
+    k = torch.randn(40, 2, 128, device="cuda").half()
+    prompt_b200.kernel(q, k, k, torch.tensor([0, 10, 30, 40], dtype=torch.int32, device="cuda"), check=True)
+    with pytest.raises(_lib.VmkDeviceStatusError) as e:
+        prompt_b200.kernel(q, k, k, torch.tensor([0, 30, 10, 40], dtype=torch.int32, device="cuda"), check=True)
+    assert e.value.status == 2
