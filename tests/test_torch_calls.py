@@ -65,7 +65,7 @@ def test_ordinary_calls_are_taken(calls):
         table, lens, refs = torch.full((4, 2), -1, dtype=torch.int32, device="cuda"), ints([0] * 4), ints([0] * 3)
         one = [pools[0]]
         if way:
-            assert calls.reserve(table, lens, refs, ints([70, 3, 0, 0]), 64).tolist() == [1, 1, 0 + 1, 1]
+            assert calls.reserve(table, lens, refs, ints([70, 3, 0, 0]), 64).tolist() == [1, 1, 1, 1]
             assert calls.append(half(73, 2, 128).zero_(), half(73, 2, 128).zero_(), pools[0], pools[0], table, ints([0, 70, 73, 73, 73]), lens)
             assert calls.compact(pools, table, lens, refs, ints([[0, 2, -1]] * 4), ints([2, 1, -1, -1]))
             assert calls.fork(tuple(one), table, lens, refs, ints([1]), ints([2]))
