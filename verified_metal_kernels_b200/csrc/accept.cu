@@ -460,16 +460,18 @@ static void accept_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2
   cfg.numAttrs = 2;
 }
 
-// CTAs per request: the most (up to 8, with at least 2048 entries each) at which the clusters of all requests are resident
-// together.  (32 requests over 131072 entries: clusters of 8 in one wave, against two waves of the same at one CTA an SM.)
+// CTAs per request: the most (up to 8, with at least 4096 entries each) at which the clusters of all requests are resident
+// together, two CTAs an SM.  Measured with at most 8, 4, 2 and 1 (us): 32 trees of 64 nodes over 131072 entries 29.9, 36.1, 57.4,
+// 97.2; one chain of 8 over 32768 6.6, 7.0, 8.2, 9.7; 32 chains of 8 over 131072 12.6, 12.1, 16.8, 26; 128 over 100003 in
+// bf16 (two are resident) 15.0 with two, 17.0 with one; 64 over 8192 (4, 2, 1) 9.2, 8.2, 7.7: hence the 4096.
 static int accept_cluster(int B, int V) {
-  if (g_batch_invariant) return V >= 4 * 2048 ? 4 : 1;    // by the row alone: the order of the sums must not follow the batch
+  if (g_batch_invariant) return V >= 4 * 4096 ? 4 : 1;    // by the row alone: the order of the sums must not follow the batch
   static std::atomic<int> resident[64][4];                 // clusters of 1 << i CTAs that run together, by device
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
   for (int i = 3; i > 0; --i) {
     const int c = 1 << i;
-    if (V < c * 2048) continue;
+    if (V < c * 4096) continue;
     int n = resident[dev][i].load();
     if (n == 0) {
       cudaLaunchConfig_t cfg;

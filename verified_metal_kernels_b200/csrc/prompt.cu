@@ -62,7 +62,10 @@ constexpr int kPmCols = 512;
 constexpr int kPmColS = 0, kPmColO = 256;
 constexpr float kPmLazy = 8.f;                   // log2 units
 constexpr int kPmPlanThreads = 1024;
-constexpr int kPmSplitMin = 4;                   // key blocks that a split is worth
+// Key blocks that a share holds at least, where 4 CTAs and more share a unit (few rows to merge) and where 2 or 3 do.  (us: 1
+// query over 512 keys 10.2 at 2, 11.2 at 4; 32 over 1500 14.1 and 15.5; 512 over 1100 26.2 at 4, 23.3 at 5; 300 over 1500
+// 25.7 at 5, 30.8 at 6; 32 heads on 8.)
+constexpr int kPmSplitFew = 2, kPmSplitMany = 5;
 constexpr int kPmMaxSplit = 32;
 constexpr int kPmBins = 256;
 constexpr int kPmMaxItems = 1 << 20;             // tiles of a call: 16 million tokens at 16 heads a group, 268 million at one
@@ -95,6 +98,7 @@ struct PromptParams {
   PromptSeqs seqs;
   int direct;                  // one unit (or one split of it) per CTA, found by the CTA itself: no planner
   int nsplit;                  // direct: CTAs that share the keys of a unit; above 1 they emit partials
+  int split_min;               // key blocks that a share holds at least
   float *part_ml, *part_o;     // [CTA][256][2], [CTA][256][128]
   const int32_t* page_table;   // paged cache: (S, table_stride); null = packed keys
   int page_size, table_stride, page_groups;
@@ -316,6 +320,7 @@ struct PromptUnit {          // what warp 8 hands to the others
   PromptItem it;
   int h;                     // kv head; -1: no more units
   int j0, na, nb;            // first key block of this CTA's share, and how many of it tiles A and B have to see
+  int parts;                 // CTAs that share the unit
   int twin;                  // both tiles hold the same rows, and take the blocks j0, j0 + 2, ... and j0 + 1, j0 + 3, ...
 };
 
@@ -331,19 +336,21 @@ __device__ __forceinline__ int tile_blocks(const PromptItem& it, int t, int tpt)
 // idle during its softmax and the other way round), and the merge joins the two like shares of their own.  Both read one Q
 // tile; the other's place is a sixth slot of the ring.  (17 tokens over 60001 keys: 62.6 us with one tile, 57.0 with two; the
 // keys alone take 38 us to read.  Asking for later blocks into L2 ahead of the ring made it 64 to 71.)
-__device__ __forceinline__ bool prompt_twin(const PromptItem& it, int tpt, int nsplit) { return nsplit > 1 && it.ntok <= tpt; }
+__device__ __forceinline__ bool prompt_twin(const PromptItem& it, int tpt, int parts) { return parts > 1 && it.ntok <= tpt; }
 
-// This CTA's share of a unit's key blocks: all of them, or part `sp` of `ns` equal ones of at least kPmSplitMin blocks.
-__device__ __forceinline__ int prompt_parts(int nblk, int nsplit) { return max(1, min(nsplit, nblk / kPmSplitMin)); }
+// This CTA's share of a unit's key blocks: all of them, or part `sp` of `nsplit` equal ones of at least split_min blocks.
+__device__ __forceinline__ int prompt_parts(int nblk, int nsplit, int split_min) { return max(1, min(nsplit, nblk / split_min)); }
 
-__device__ __forceinline__ void prompt_share(PromptUnit& u, int tpt, int nsplit, int sp) {
+__device__ __forceinline__ void prompt_share(PromptUnit& u, int tpt, int nsplit, int split_min, int sp) {
   const int na = tile_blocks(u.it, 0, tpt), nb = tile_blocks(u.it, 1, tpt), nblk = max(na, nb);
-  const int parts = prompt_parts(nblk, nsplit);
+  const int parts = prompt_parts(nblk, nsplit, split_min);
+  u.parts = parts;
+  if (sp >= parts) u.h = -1;
   const int j0 = sp < parts ? (int)((long long)nblk * sp / parts) : nblk, j1 = sp < parts ? (int)((long long)nblk * (sp + 1) / parts) : nblk;
   u.j0 = j0;
   u.na = max(0, min(na, j1) - j0);
   u.nb = max(0, min(nb, j1) - j0);
-  u.twin = prompt_twin(u.it, tpt, nsplit);
+  u.twin = prompt_twin(u.it, tpt, parts);
   if (u.twin) {
     u.nb = u.na / 2;
     u.na -= u.nb;
@@ -441,7 +448,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
         PromptUnit un;
         un.it = prompt_item(p.seqs, q0, nq, k0, nk, t);
         un.h = un.it.h = u % p.Hkv;
-        prompt_share(un, p.tpt, p.nsplit, sp);
+        prompt_share(un, p.tpt, p.nsplit, p.split_min, sp);
         units[0] = un;
         if (p.nsplit > 1 && sp == 0) p.items[u] = un.it;
       }
@@ -476,7 +483,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
         } else if (u < n_units) {
           un.it = p.items[u / p.Hkv];
           un.h = u % p.Hkv;
-          prompt_share(un, p.tpt, 1, 0);
+          prompt_share(un, p.tpt, 1, 1, 0);
         }
         units[sl] = un;
         mbar_arrive(&sched_full[sl]);
@@ -719,7 +726,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
       if (!__all_sync(0xffffffffu, mbar_wait(&sched_full[sl], (n / kPmSched) & 1))) { timed_out = true; break; }
       const PromptItem it = units[sl].it;
       const int h = units[sl].h, j0 = units[sl].j0, na = units[sl].na, nb = units[sl].nb;
-      const bool twin = SPLIT && units[sl].twin;
+      const bool twin = SPLIT && units[sl].twin, part = SPLIT && units[sl].parts > 1;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sched_empty[sl]);
       if (h < 0) break;
@@ -839,7 +846,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
         if (!__all_sync(0xffffffffu, mbar_wait(&o_full[t], n_o++ & 1))) { timed_out = true; break; }
         tc_fence_after();
       }
-      if constexpr (SPLIT) {
+      if (part) {
         // a share of the keys: the row's maximum, sum and unnormalised output, for the merge
         const size_t at = (size_t)blockIdx.x * 256 + t * 128 + row;
         if (valid) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mine > 0 ? m : -INFINITY, l);
@@ -896,16 +903,19 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
   }
 }
 
-// Merge of a unit's shares: one warp per row, four columns per lane.
-__global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptParams p) {
+// Merge of a unit's shares: one warp per row, four columns per lane; K shares (of two tiles each, where both hold the row) are
+// loaded at a time: many where few rows have many shares, few where many rows need the registers.
+template <int K>
+__global__ void __launch_bounds__(256, K > 2 ? 2 : 6) prompt_merge_kernel(const PromptParams p) {
   const int lane = threadIdx.x & 31;
   const int u = blockIdx.x >> 5, r = (blockIdx.x & 31) * 8 + (threadIdx.x >> 5);       // row of the 256
   pdl_wait();
   const PromptItem it = p.items[u];
   const int t = r >> 7, tok = (r & 127) / p.G, g = (r & 127) - tok * p.G, tk = t * p.tpt + tok;
   if (tok >= p.tpt || tk >= it.ntok) return;
-  const int parts = prompt_parts(max(tile_blocks(it, 0, p.tpt), tile_blocks(it, 1, p.tpt)), p.nsplit);
-  const int tiles = prompt_twin(it, p.tpt, p.nsplit) ? 2 : 1;     // of a share that hold this row
+  const int parts = prompt_parts(max(tile_blocks(it, 0, p.tpt), tile_blocks(it, 1, p.tpt)), p.nsplit, p.split_min);
+  if (parts == 1) return;                                // it has its result
+  const int tiles = prompt_twin(it, p.tpt, parts) ? 2 : 1;     // of a share that hold this row
   const size_t at0 = (size_t)u * p.nsplit * 256 + r;
   float2 ml[2];
   float m = -INFINITY;
@@ -926,11 +936,11 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptParams p)
   l = warp_sum(l);
   const float scale = l > 0.f || l != l ? 1.f / l : 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = 0; i < parts; i += 8) {                   // (loads under predicates: sixteen are in flight)
-    float4 v[8][2];
-    float wi[8][2];
+  for (int i = 0; i < parts; i += K) {                   // (loads under predicates: all of them in flight)
+    float4 v[K][2];
+    float wi[K][2];
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         wi[k][s] = __shfl_sync(0xffffffffu, w[s], (i + k) & 31);
@@ -940,7 +950,7 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptParams p)
         if (wi[k][s] != 0.f) v[k][s] = *reinterpret_cast<const float4*>(p.part_o + (at0 + (size_t)(i + k) * 256 + s * 128) * kPmD + lane * 4);
       }
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         o.x += wi[k][s] * v[k][s].x;
@@ -963,11 +973,14 @@ static int prompt_tiles_bound(int Tq, int S, int tpt) {
   return n > kPmMaxItems ? -1 : (int)n;
 }
 
-// How a call is cut.  Up to one unit per SM, every CTA finds its unit itself, and where that leaves half of the SMs or more
-// without one, several CTAs share a unit's keys (few rows over a long cache are bound by how many SMs read it).  Else
-// the planner's list and persistent CTAs.  The batch-invariant mode never splits: how many share depends on the batch.
+// How a call is cut.  Up to one unit per SM, every CTA finds its unit itself (one prompt of 128 tokens 9.3 us, with the planner
+// 12.4; of 1000 tokens 22.8 and 25.3), and where that leaves half of the SMs or more without one, several CTAs share a unit's
+// keys: few rows over a long cache are bound by how many SMs read it (17 queries over 9000 keys 17.8 us, not shared 108.8;
+// 1 over 1000 10.4 and 17.4; 512 over 4000 44.4 and 61.5; where no unit turns out to be worth sharing, the merge's launch is lost: four
+// of 64 over 700 22.3 and 19.2).  Else the planner's list and persistent CTAs.  The batch-invariant mode never shares: how
+// many CTAs do depends on the batch.
 struct PromptPlan {
-  int max_items, direct, nsplit, grid;
+  int max_items, direct, nsplit, split_min, grid;
   size_t items_bytes, ws_bytes;
 };
 
@@ -977,11 +990,12 @@ static bool prompt_plan(PromptPlan& pl, int S, int Tq, long long keys, int Hkv, 
   const long long units = (long long)pl.max_items * Hkv;
   const int sms = sm_count();
   pl.direct = units <= sms;
-  pl.nsplit = 1;
+  pl.nsplit = pl.split_min = 1;
   if (pl.direct && !g_batch_invariant && units > 0) {
     // what prompt_parts can come to for a sequence of all the keys: the bound changes no result, only the scratch
-    const long long most = (keys + kPmBK - 1) / kPmBK / kPmSplitMin;
     pl.nsplit = (int)(sms / units);
+    pl.split_min = pl.nsplit >= 4 ? kPmSplitFew : kPmSplitMany;
+    const long long most = (keys + kPmBK - 1) / kPmBK / pl.split_min;
     if (pl.nsplit > most) pl.nsplit = (int)most;
     if (pl.nsplit > kPmMaxSplit) pl.nsplit = kPmMaxSplit;
     if (pl.nsplit < 2) pl.nsplit = 1;
@@ -1055,6 +1069,7 @@ static int prompt_impl(const void* q, const void* k, const void* v, const int32_
   p.part_o = p.part_ml + (size_t)pl.grid * 256 * 2;
   p.direct = pl.direct;
   p.nsplit = pl.nsplit;
+  p.split_min = pl.split_min;
   p.page_table = paged ? page_table : nullptr;
   p.page_size = page_size;
   p.table_stride = table_stride;
@@ -1099,10 +1114,11 @@ static int prompt_impl(const void* q, const void* k, const void* v, const int32_
                                     : (bf16 ? prompt_kernel<true, false> : prompt_kernel<false, false>);
   rc = check_launch(cudaLaunchKernelEx(&cfg, kernel, p));
   if (rc != VMK_OK || pl.nsplit == 1) return rc;
+  // (17 queries over 60001 keys 51.6 us with eight shares at a time, 54.2 with two; 512 over 2000 48.8 and 31.8)
   cfg.gridDim = dim3(pl.grid / pl.nsplit * 32);
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
-  return check_launch(cudaLaunchKernelEx(&cfg, prompt_merge_kernel, p));
+  return check_launch(cudaLaunchKernelEx(&cfg, pl.nsplit >= 4 ? prompt_merge_kernel<8> : prompt_merge_kernel<2>, p));
 }
 
 }  // namespace vmk
