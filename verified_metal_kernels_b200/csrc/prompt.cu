@@ -272,6 +272,26 @@ __device__ __forceinline__ void pm_store32(void* dst, const uint32_t (&w)[8]) { 
                "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
 }
+// 16 lanes x 64 columns of tensor memory: r[4 i .. 4 i + 1] are columns 8 i + 2 (lane % 4) + {0, 1} of row lane / 4, the other two
+// those of row lane / 4 + 8.
+__device__ __forceinline__ void pm_tmem_ld_16x64(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+               : "r"(taddr));
+}
+// Four lanes hold four words each: word e of lane l and word l of lane e change places.
+__device__ __forceinline__ void pm_quad_transpose(uint32_t (&v)[4], int lane) {
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    const bool up = (lane & o) != 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (k & o) continue;
+      const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? v[k] : v[k + o], o);
+      if (up) v[k] = got; else v[k + o] = got;
+    }
+  }
+}
 __device__ __forceinline__ float pm_max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -870,24 +890,42 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
         continue;
       }
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;           // 0: the row saw no key (a NaN stays one)
-      __half* dst = p.out + ((size_t)(it.tok0 + tk) * p.Hq + (size_t)h * p.G + g) * kPmD;
-      // (a thread has a row: 32-byte stores fill whole sectors, which 16-byte ones at twice the number did not: a warp's
-      // store of 32 rows takes the load/store unit 32 cycles whatever its width)
+      const unsigned long long dst =
+          valid ? (unsigned long long)(p.out + ((size_t)(it.tok0 + tk) * p.Hq + (size_t)h * p.G + g) * kPmD) : 0ull;
+      // Whole 128-byte lines: a quad of lanes has 64 columns of a row (8 rows a store).  With a row to each thread (32 sectors of as
+      // many lines a store) the stores took 2 us a unit, and all that followed in the load/store unit waited for them.
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        const int la = half * 16 + (lane >> 2);
+        const float ia = __shfl_sync(0xffffffffu, inv, la), ib = __shfl_sync(0xffffffffu, inv, la + 8);
+        const unsigned long long da = __shfl_sync(0xffffffffu, dst, la), db = __shfl_sync(0xffffffffu, dst, la + 8);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t o[32];
-        if (mine > 0) {
-          tmem_ld32(tO + c * 32, o);
-          tmem_ld_wait();
-        }
-        if (!valid) continue;
+        for (int c = 0; c < 2; ++c) {
+          uint32_t o[32], wa[8], wb[8];
+          if (mine > 0) {
+            pm_tmem_ld_16x64(tO + ((uint32_t)(half * 16) << 16) + c * 64, o);
+            tmem_ld_wait();
+          }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t w[8];
+          for (int x = 0; x < 2; ++x) {
+            uint32_t ta[4], tb[4];
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            w[e] = mine > 0 && inv != 0.f ? pack2(__uint_as_float(o[16 * i + 2 * e]) * inv, __uint_as_float(o[16 * i + 2 * e + 1]) * inv, BF) : 0u;
-          pm_store32(dst + c * 32 + i * 16, w);
+            for (int e = 0; e < 4; ++e) {
+              const int i = 4 * (2 * e + x);
+              ta[e] = mine > 0 && ia != 0.f ? pack2(__uint_as_float(o[i]) * ia, __uint_as_float(o[i + 1]) * ia, BF) : 0u;
+              tb[e] = mine > 0 && ib != 0.f ? pack2(__uint_as_float(o[i + 2]) * ib, __uint_as_float(o[i + 3]) * ib, BF) : 0u;
+            }
+            pm_quad_transpose(ta, lane);
+            pm_quad_transpose(tb, lane);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              wa[4 * x + e] = ta[e];
+              wb[4 * x + e] = tb[e];
+            }
+          }
+          const int at = (c * 64 + (lane & 3) * 16) * 2;
+          if (da != 0ull) pm_store32(reinterpret_cast<uint8_t*>(da) + at, wa);
+          if (db != 0ull) pm_store32(reinterpret_cast<uint8_t*>(db) + at, wb);
         }
       }
       tc_fence_before();                                  // these loads before the p_full of the next unit
