@@ -31,7 +31,7 @@
 // sum that divides is that of the unrounded P.
 //
 // Measured (bf16, 32 query heads on 8): 32768 tokens 6.6 ms on a cool GPU (1330 TFLOP/s over the visible pairs), 7.4 to 7.7 at
-// the power limit (1.55 to 1.7 GHz); 24 prompts of up to 1999 tokens 246 us; 128 tokens 8.9 us; 17 tokens over 60001 keys 52
+// the power limit (1.55 to 1.7 GHz); 24 prompts of up to 1999 tokens 239 us; 128 tokens 8.7 us; 17 tokens over 60001 keys 52
 // to 57 us (4.3 to 4.7 TB/s).  What bounds the long ones: each tile's softmax and products follow one another, and two tiles
 // keep the tensor pipe and the exponential unit at about 60 % each.  A block of 128 keys costs a pair of tiles 3500 cycles
 // where the products alone take 2060 and the exponentials 2048.  Tried, and slower: scores of 64 keys in two buffers (N = 64
@@ -893,7 +893,8 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
       const unsigned long long dst =
           valid ? (unsigned long long)(p.out + ((size_t)(it.tok0 + tk) * p.Hq + (size_t)h * p.G + g) * kPmD) : 0ull;
       // Whole 128-byte lines: a quad of lanes has 64 columns of a row (8 rows a store).  With a row to each thread (32 sectors of as
-      // many lines a store) the stores took 2 us a unit, and all that followed in the load/store unit waited for them.
+      // many lines a store) the load/store unit was busy with a unit's stores for 2 us, now for 1.4 (24 ragged prompts 244.6 ->
+      // 238.8 us).  Loading more of O at a time spills.
 #pragma unroll 1
       for (int half = 0; half < 2; ++half) {
         const int la = half * 16 + (lane >> 2);
