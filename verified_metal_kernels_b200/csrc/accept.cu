@@ -163,9 +163,11 @@ __device__ __forceinline__ void ac_weights(float (&hi)[AcVec<T>::N], float (&lo)
   } else {
     for (int g = 0; g < n_gone; ++g) {
       const int k0 = gone[g] - e0;
+      if ((unsigned)k0 < (unsigned)N) {
 #pragma unroll
-      for (int k = 0; k < N; ++k)
-        if (k == k0) hi[k] = 0.f;
+        for (int k = 0; k < N; ++k)
+          if (k == k0) hi[k] = 0.f;
+      }
     }
   }
 }
