@@ -22,6 +22,15 @@ def test_build_is_keyed_by_content(calls):
     assert build.build_calls() == build.CALLS_LIB and os.stat(build.CALLS_LIB).st_mtime_ns == before
 
 
+def test_kernels_are_reached_by_name():
+    from verified_metal_kernels_b200 import load_kernel
+    from verified_metal_kernels_b200.kernels import decode_b200
+    assert load_kernel("prompt") is prompt_b200.kernel and load_kernel("accept") is accept_b200.kernel
+    assert load_kernel("decode") is decode_b200.kernel
+    with pytest.raises(KeyError):
+        load_kernel("pages")                   # several functions: kernels.pages_b200
+
+
 def test_calls_that_are_not_ordinary_are_handed_back(calls):
     t, i = torch.zeros(4, 2, 128, dtype=torch.float16), torch.zeros(2, dtype=torch.int32)
     table, pool = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(3, 2, 64, 128, dtype=torch.float16)

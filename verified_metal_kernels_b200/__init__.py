@@ -1,4 +1,5 @@
-"""B200-native (sm_100a) implementation of the attention-decode ops `prefix`, `spec` and `dsa`.
+"""B200-native (sm_100a) implementation of the attention-decode ops `prefix`, `spec` and `dsa`, and of what a server runs
+around them: plain decode, attention of prompts, acceptance of drafts, the pages of the cache (kernels/pages_b200.py).
 
     ops/      the op contract: shapes, seeded input generators, standard-op opponents
     kernels/  one module per op exposing `kernel(...)` with the reference signature
@@ -10,7 +11,10 @@ from . import ops  # noqa: F401
 
 KERNEL_MODULES = {"prefix": "verified_metal_kernels_b200.kernels.prefix_b200",
                   "spec": "verified_metal_kernels_b200.kernels.spec_b200",
-                  "dsa": "verified_metal_kernels_b200.kernels.dsa_b200"}
+                  "dsa": "verified_metal_kernels_b200.kernels.dsa_b200",
+                  "decode": "verified_metal_kernels_b200.kernels.decode_b200",
+                  "prompt": "verified_metal_kernels_b200.kernels.prompt_b200",
+                  "accept": "verified_metal_kernels_b200.kernels.accept_b200"}
 
 
 def load_kernel(opname):
