@@ -272,8 +272,8 @@ VMK_API int vmk_dsa_index_project(const void* x, const void* wq, const void* ww,
  *   strides (6 int64 in HOST memory, nullable): token and head strides in elements of q, k and v (the innermost axis
  *   is contiguous); positive multiples of 8.  Null: C-contiguous.  out is C-contiguous and
  *   32-byte aligned.
- *   Keys of other sequences and behind the last one may hold anything.  A NaN or infinity in v INSIDE a sequence
- *   reaches the rows that see it, and may reach rows before it whose last block of 128 keys holds it.
+ *   Keys of other sequences and behind the last one may hold anything.  A NaN or infinity in k or v inside a sequence
+ *   reaches the rows that see its key and no other (in v: the column that it stands in).
  * vmk_prompt_paged reads the keys of sequence s from the pages of page_table[s] as vmk_decode_paged does: k_pages,
  * v_pages (pages,Hkv,page_size,D), page_size a multiple of 64, lens (S) int32 = nk (the new tokens included);
  * strides holds the two of q.  A page id outside [0, pages) reads as zeros.

@@ -337,3 +337,38 @@ def test_a_short_list_that_does_not_ascend_is_reported():
     with pytest.raises(_lib.VmkDeviceStatusError) as e:
         prompt_b200.kernel(q, k, k, torch.tensor([0, 30, 10, 40], dtype=torch.int32, device="cuda"), check=True)
     assert e.value.status == 2
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("seqs", [[(300, 300)], [(40, 1100)], [(9, 1500), (70, 500)], [(513, 513)] * 3, [(100, 100)] * 40, [(5, 5)]], ids=str)
+def test_special_values_in_v_reach_the_rows_that_see_them_and_no_other(seqs, dtype):
+    """NaN in one column and infinity in another, at keys that rows before them share a block with: every other element
+    keeps its bits, packed or paged, shared by several CTAs or not."""
+    inp = _inputs(seqs, 8, 2, dtype, seed=103)
+    d = _dev(inp, dtype)
+    nk = [m for _, m in seqs]
+    rng = np.random.default_rng(5)
+    v, hit = inp["v"].copy(), []
+    for s, (nq, m) in enumerate(seqs):
+        for at in sorted({m - 1, m - 2, m - nq, int(rng.integers(m - nq, m)), int(rng.integers(0, m))}):
+            col, head = int(rng.integers(0, 128)), int(rng.integers(0, 2))
+            v[sum(nk[:s]) + at, head, col] = rng.choice([np.nan, np.inf, -np.inf])
+            hit.append((s, at, head, col))
+
+    def run(v):
+        kp, vp, table = op.to_pages(inp["k"].astype(np.float32), np.asarray(v, dtype=np.float32), nk, 64, seed=4)
+        paged = prompt_b200.kernel_paged(d["q"], torch.from_numpy(kp).cuda().to(dtype), torch.from_numpy(vp).cuda().to(dtype), torch.from_numpy(table).cuda(),
+                                         d["cu_q"], torch.tensor(nk, dtype=torch.int32, device="cuda"), check=True)
+        return prompt_b200.kernel(**{**d, "v": torch.from_numpy(np.ascontiguousarray(v)).cuda().to(dtype)}, check=True), paged
+
+    clean, _ = run(inp["v"])
+    for out in run(v):
+        want = clean.float()
+        for s, at, head, col in hit:
+            nq, m = seqs[s]
+            q0 = sum(n for n, _ in seqs[:s])
+            first = max(0, at - (m - nq))
+            want[q0 + first:q0 + nq, head * 4:head * 4 + 4, col] += float(v[sum(nk[:s]) + at, head, col])
+        same = torch.isfinite(want)
+        assert torch.equal(out.float()[same], want[same])
+        assert (torch.isnan(out.float()[~same]) | (out.float()[~same] == want[~same])).all() and not torch.isfinite(out.float()[~same]).any()

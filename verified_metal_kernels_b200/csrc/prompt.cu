@@ -23,7 +23,8 @@
 //               overwrite the scores of a block as soon as the P.V that reads their P is issued: no wait between the
 //               two, and the pipe runs one tile's pair while the other tile's softmax works
 //   warps 0-3   softmax of tile A, warps 4-7 of tile B: one thread per row
-//   warp 10     zeroes the rows of `out` outside every sequence (warp 11 only completes the warp group)
+//   warps 10,11 look for NaN and infinities in the rows of V that not every row of the unit sees; warp 10 zeroes the rows of `out`
+//               outside every sequence
 // Tensor memory (512 columns): S_A, S_B, O_A, O_B, 128 columns each; P (16-bit pairs, 64 columns) over its scores.
 // O is rescaled only when a row's maximum grew by more than 2^8 (P stays below 2^8 and the result is exact); the
 // softmax thread does it itself: when the scores of block j are there, the P.V of block j - 1, issued before them,
@@ -31,13 +32,16 @@
 // sum that divides is that of the unrounded P.
 //
 // Measured (bf16, 32 query heads on 8): 32768 tokens 6.6 ms on a cool GPU (1330 TFLOP/s over the visible pairs), 7.4 to 7.7 at
-// the power limit (1.55 to 1.7 GHz); 24 prompts of up to 1999 tokens 239 us; 128 tokens 8.7 us; 17 tokens over 60001 keys 52
+// the power limit (1.55 to 1.7 GHz); 24 prompts of up to 1999 tokens 247 us; 128 tokens 8.8 us; 17 tokens over 60001 keys 52
 // to 57 us (4.3 to 4.7 TB/s).  What bounds the long ones: each tile's softmax and products follow one another, and two tiles
 // keep the tensor pipe and the exponential unit at about 60 % each.  A block of 128 keys costs a pair of tiles 3500 cycles
 // where the products alone take 2060 and the exponentials 2048.  Tried, and slower: scores of 64 keys in two buffers (N = 64
 // products take 48 cycles, not 32), two threads a row, warps of their own for the result, a polynomial for a quarter of the
 // exponentials, products cut to the keys that a tile's last block has (the descriptors then leave the uniform registers).
 //
+// A key that a row does not see has P = 0, but 0 times Inf or NaN is NaN.  In the blocks that the mask cuts, such entries of V
+// are cleared in shared memory and added to the results of the rows that see their key (prompt_add_special).  (One short prompt
+// 8.67 -> 8.75 us, 24 ragged ones 237 -> 247, a long one the same; one warp a tile instead of two that share the rows 9.27 and 245.)
 // Rows of V past the end of a sequence (the next sequence's, or whatever a page holds there) are cleared in shared
 // memory before the product: their P is 0, but 0 times Inf would poison the row.
 // Every mbarrier wait is bounded; a wait that runs out sets the status word and the CTA winds down through the common
@@ -103,6 +107,8 @@ struct PromptParams {
   const int32_t* page_table;   // paged cache: (S, table_stride); null = packed keys
   int page_size, table_stride, page_groups;
   int Tq, Hq, Hkv, G, tpt;     // tpt = tokens per 128-row tile
+  const uint16_t* v;           // as tmV describes it
+  long long v_tok, v_head;     // packed: strides in elements
   float sc;                    // log2(e) / sqrt(128)
   int bf16;
   int32_t* status;
@@ -378,8 +384,52 @@ __device__ __forceinline__ void prompt_share(PromptUnit& u, int tpt, int nsplit,
 }
 
 constexpr int kPmBars = 2 * kPmTwinSlots + 2 * kPmSched + 2 + 2 + 2 + 2 + 2 + 2 + 2;   // (an even number: what follows is 16-byte aligned)
-constexpr int kPmSmem = 2 * kPmTile + kPmSlots * kPmTile + kPmBars * 8 + kPmSched * (int)sizeof(PromptUnit) + 16 + 1024;
+constexpr int kPmSpecial = 4;                    // units that a flag of theirs has to outlive, and more
+constexpr int kPmSmem =
+    2 * kPmTile + kPmSlots * kPmTile + kPmBars * 8 + kPmSched * (int)sizeof(PromptUnit) + 16 + 2 * kPmSpecial * 4 + 1024;
 static_assert(kPmSmem <= 232448, "shared memory of one CTA");
+
+// NaN and infinite, in either 16-bit type.
+template <bool BF>
+__device__ __forceinline__ bool pm_special(uint32_t h) { return BF ? (h & 0x7f80u) == 0x7f80u : (h & 0x7c00u) == 0x7c00u; }
+template <bool BF>
+__device__ __forceinline__ float pm_float(uint16_t h) {
+  return BF ? __uint_as_float((uint32_t)h << 16) : __half2float(__ushort_as_half(h));
+}
+
+template <bool BF>
+__device__ __forceinline__ void pm_times_zero(uint32_t& acc, uint32_t x) {
+  if (BF) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(x), "r"(0u));
+  else asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(x), "r"(0u));
+}
+
+// Adds the NaN and infinite entries of V at keys [k0, k1) of a unit's sequence to a row that sees them all: to its result, or to its share.
+template <bool BF, bool PART>
+__device__ __forceinline__ void prompt_add_special(const PromptParams& p, const PromptItem& it, int h, int k0, int k1, void* row) {
+#pragma unroll 1
+  for (int x = k0; x < k1; ++x) {
+    const uint16_t* v = nullptr;
+    if (p.page_table == nullptr) {
+      v = p.v + (long long)(it.k0 + x) * p.v_tok + (long long)h * p.v_head;
+    } else {
+      const int id = x / p.page_size < p.table_stride ? p.page_table[(size_t)it.k0 * p.table_stride + x / p.page_size] : -1;
+      if (id >= 0 && id < p.page_groups / p.Hkv) v = p.v + (((size_t)id * p.Hkv + h) * p.page_size + x % p.page_size) * kPmD;
+    }
+    if (v == nullptr) continue;
+#pragma unroll 1
+    for (int c = 0; c < kPmD; ++c) {
+      const uint16_t e = v[c];
+      if (!pm_special<BF>(e)) continue;
+      if (PART) {
+        static_cast<float*>(row)[c] += pm_float<BF>(e);
+      } else {
+        uint16_t* o = static_cast<uint16_t*>(row) + c;
+        const float sum = pm_float<BF>(*o) + pm_float<BF>(e);
+        *o = (uint16_t)pack2(sum, 0.f, BF);
+      }
+    }
+  }
+}
 
 // SPLIT: CTAs share units' keys and emit partials (always direct: one unit each).  An instance of its own, so that the
 // loops of the others hold nothing of it.
@@ -392,16 +442,17 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
   uint64_t* full = reinterpret_cast<uint64_t*>(sKV + kPmSlots * kPmTile);   // K or V tile landed (TMA bytes)
   uint64_t* empty = full + kPmTwinSlots;                 // consumed by both tiles' products   (MMA commit)
   uint64_t* sched_full = empty + kPmTwinSlots;           // unit written                       (warp 8)
-  uint64_t* sched_empty = sched_full + kPmSched;         // unit read by everybody             (9 warps)
+  uint64_t* sched_empty = sched_full + kPmSched;         // unit read by everybody             (11 warps)
   uint64_t* q_full = sched_empty + kPmSched;             // [tile] Q tile landed               (TMA bytes)
   uint64_t* q_empty = q_full + 2;                        // [tile] last Q.K^T of a unit done   (MMA commit)
   uint64_t* s_full = q_empty + 2;                        // [tile] scores ready                (MMA commit)
-  uint64_t* p_part = s_full + 2;                         // [tile] P of the first 96 keys in tensor memory (4 warps)
+  uint64_t* p_part = s_full + 2;                         // [tile] P of the first 96 keys in tensor memory, V looked at (6 warps)
   uint64_t* p_full = p_part + 2;                         // [tile] all of P                    (4 warps)
   uint64_t* o_full = p_full + 2;                         // [tile] last P.V of a unit done     (MMA commit)
   uint64_t* drain = o_full + 2;                          // every product done, after a timeout
   PromptUnit* units = reinterpret_cast<PromptUnit*>(sKV + kPmSlots * kPmTile + kPmBars * 8);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(units + kPmSched);
+  uint32_t* special = tmem_slot + 4;                     // [unit % 4][warp 10, 11]: 1 + the unit, if it cleared entries of V
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -411,17 +462,18 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
     }
     for (int s = 0; s < kPmSched; ++s) {
       mbar_init(&sched_full[s], 1);
-      mbar_init(&sched_empty[s], 9);
+      mbar_init(&sched_empty[s], 11);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_part[t], 4);
+      mbar_init(&p_part[t], 6);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_full[t], 1);
     }
     mbar_init(drain, 1);
+    for (int i = 0; i < 2 * kPmSpecial; ++i) special[i] = 0u;
     fence_mbar_init();
   }
   if (warp == 9) tmem_alloc(tmem_slot, kPmCols);
@@ -720,15 +772,72 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
       pm_commit(lead, drain);
       mbar_wait(drain, 0);
     }
-  } else if (warp == 10) {
-    // ------------------------------------------------------------------------------ rows outside every sequence
-    const int lo = min(max(p.seqs.cu_q[0], 0), p.Tq);
-    const int hi = max(lo, min(max(p.seqs.cu_q[p.seqs.S], 0), p.Tq));
-    const size_t row16 = (size_t)p.Hq * (kPmD / 8);       // 16-byte chunks of one token's row
-    const size_t n = (size_t)(lo + (p.Tq - hi)) * row16;
-    for (size_t e = (size_t)blockIdx.x * 32 + lane; e < n; e += (size_t)gridDim.x * 32) {
-      const size_t at = e < (size_t)lo * row16 ? e : e - (size_t)lo * row16 + (size_t)hi * row16;
-      reinterpret_cast<uint4*>(p.out)[at] = make_uint4(0u, 0u, 0u, 0u);
+  } else {
+    // ------------------------------------------------------------------------------ NaN and infinities in V
+    const int mine = warp - 10;                            // the two share a block's rows
+    uint32_t ring = 0, n_p[2] = {0, 0};
+    for (uint32_t n = 0; !timed_out; ++n) {
+      const int sl = n % kPmSched;
+      if (!__all_sync(0xffffffffu, mbar_wait(&sched_full[sl], (n / kPmSched) & 1))) { timed_out = true; break; }
+      const int h = units[sl].h, j0 = units[sl].j0, na = units[sl].na, nb = units[sl].nb, nk = units[sl].it.nk, vis0 = units[sl].it.vis0;
+      const bool twin = SPLIT && units[sl].twin;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sched_empty[sl]);
+      if (h < 0) break;
+      const int nblk = twin ? na + nb : max(na, nb);
+      const int vis_all = min(nk, max(0, vis0 + 1));       // keys that the unit's first token sees
+      for (int j = 0; j < nblk && !timed_out; ++j) {
+        const int kb = (j0 + j) * kPmBK, r0 = max(0, vis_all - kb), r1 = min(kPmBK, nk - kb);
+        if (r0 < r1) {
+          const uint32_t iv = ring + 2 * j + 1, slots = twin ? kPmTwinSlots : kPmSlots;
+          if (!__all_sync(0xffffffffu, mbar_wait(&full[iv % slots], (iv / slots) & 1))) { timed_out = true; break; }
+          uint8_t* v = sKV + (iv % slots) * kPmTile - (twin ? kPmTile : 0);
+          // 0 x + 0 is NaN where x is NaN or infinite, and 0 or -0 elsewhere: one packed product for two entries
+          uint32_t acc[4] = {0u, 0u, 0u, 0u};
+          const uint8_t* col = v + ((lane & 15) >> 3) * kPmHalf;
+          const int first = r0 + 2 * mine + (lane >> 4);
+#pragma unroll 8
+          for (int r = first; r < r1; r += 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(col + swz128(r, lane & 7));
+            pm_times_zero<BF>(acc[0], x.x);
+            pm_times_zero<BF>(acc[1], x.y);
+            pm_times_zero<BF>(acc[2], x.z);
+            pm_times_zero<BF>(acc[3], x.w);
+          }
+          if (__any_sync(0xffffffffu, ((acc[0] | acc[1] | acc[2] | acc[3]) & 0x7fff7fffu) != 0u)) {
+            if (lane == 0) *reinterpret_cast<volatile uint32_t*>(special + (n % kPmSpecial) * 2 + mine) = n + 1;
+#pragma unroll 1
+            for (int r = first; r < r1; r += 4)
+#pragma unroll 1
+              for (int c = 0; c < 8; ++c) {
+                uint16_t* x = reinterpret_cast<uint16_t*>(v + ((lane & 15) >> 3) * kPmHalf + swz128(r, lane & 7)) + c;
+                if (pm_special<BF>(*x)) *x = 0;
+              }
+          }
+          fence_proxy_async();
+          __syncwarp();
+        }
+        // each tile that the block belongs to; an arrival counts for the phase after the one that is complete
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (twin ? (j & 1) != t : j >= (t == 0 ? na : nb)) continue;
+          if (n_p[t] > 0 && !__all_sync(0xffffffffu, mbar_wait(&p_part[t], (n_p[t] - 1) & 1))) { timed_out = true; continue; }
+          if (lane == 0) mbar_arrive(&p_part[t]);
+          ++n_p[t];
+        }
+      }
+      ring += 2 * nblk;
+    }
+    if (warp == 10) {
+      // ------------------------------------------------------------------------------ rows outside every sequence
+      const int lo = min(max(p.seqs.cu_q[0], 0), p.Tq);
+      const int hi = max(lo, min(max(p.seqs.cu_q[p.seqs.S], 0), p.Tq));
+      const size_t row16 = (size_t)p.Hq * (kPmD / 8);       // 16-byte chunks of one token's row
+      const size_t n = (size_t)(lo + (p.Tq - hi)) * row16;
+      for (size_t e = (size_t)blockIdx.x * 32 + lane; e < n; e += (size_t)gridDim.x * 32) {
+        const size_t at = e < (size_t)lo * row16 ? e : e - (size_t)lo * row16 + (size_t)hi * row16;
+        reinterpret_cast<uint4*>(p.out)[at] = make_uint4(0u, 0u, 0u, 0u);
+      }
     }
   }
   } else {
@@ -866,6 +975,10 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
         if (!__all_sync(0xffffffffu, mbar_wait(&o_full[t], n_o++ & 1))) { timed_out = true; break; }
         tc_fence_after();
       }
+      // entries of V that were cleared, at keys that this row sees: those behind the first that not all rows of the unit see
+      const volatile uint32_t* sp = special + (n % kPmSpecial) * 2;
+      const bool add = sp[0] == n + 1 || sp[1] == n + 1;
+      const int add0 = max(min(it.nk, max(0, it.vis0 + 1)), j0 * kPmBK), add1 = min(vis, (j0 + nblk) * kPmBK);
       if (part) {
         // a share of the keys: the row's maximum, sum and unnormalised output, for the merge
         const size_t at = (size_t)blockIdx.x * 256 + t * 128 + row;
@@ -886,6 +999,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
             }
           }
         }
+        if (add && valid && mine > 0) prompt_add_special<BF, true>(p, it, h, add0, add1, p.part_o + at * kPmD);
         tc_fence_before();
         continue;
       }
@@ -928,6 +1042,10 @@ __global__ void __launch_bounds__(kPmThreads, 1) prompt_kernel(const __grid_cons
           if (da != 0ull) pm_store32(reinterpret_cast<uint8_t*>(da) + at, wa);
           if (db != 0ull) pm_store32(reinterpret_cast<uint8_t*>(db) + at, wb);
         }
+      }
+      if (add) {
+        __syncwarp();
+        if (valid && mine > 0) prompt_add_special<BF, false>(p, it, h, add0, add1, reinterpret_cast<void*>(dst));
       }
       tc_fence_before();                                  // these loads before the p_full of the next unit
     }
@@ -1111,6 +1229,9 @@ static int prompt_impl(const void* q, const void* k, const void* v, const int32_
   p.split_min = pl.split_min;
   p.page_table = paged ? page_table : nullptr;
   p.page_size = page_size;
+  p.v = static_cast<const uint16_t*>(v);
+  p.v_tok = sv.tok;
+  p.v_head = sv.head;
   p.table_stride = table_stride;
   p.page_groups = paged ? pages * Hkv : 0;
   p.Tq = Tq;
