@@ -316,7 +316,9 @@ VMK_API int vmk_accept(const void* target_probs, const void* draft_probs, const 
  *   pools: HOST array of four int64 per pool: device address (16-byte aligned), layers, heads, bytes of one position of
  *   one head (a multiple of 16): a contiguous tensor (layers, pages, heads, page_size, bytes).  Up to 8 pools.
  * vmk_pages_reserve: row r grows by extra[r] >= 0 positions: gets the pages, lens[r] += extra[r].  granted (R), nullable: 1
- *   or 0.  A row whose table would be too short is refused (status bit 2).
+ *   or 0.  A row whose table would be too short is refused (status bit 2), and so is one whose last page is partly used and
+ *   named by other slots as well (vmk_pages_free cut it there, or a row forked from it goes on there): its next positions
+ *   are theirs.  vmk_pages_fork of such a row into an empty one gives it a page of its own.
  * vmk_pages_append: writes tokens into two pools of one layer each (keys and values): sources = HOST array of three
  *   int64 for each: address, token stride and head stride in bytes (multiples of 16).  Token t of the packed tokens
  *   [cu[s], cu[s+1]) of row s goes to position lens[s] - (cu[s+1] - t): lens counts the new tokens already.  Tokens

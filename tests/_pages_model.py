@@ -14,11 +14,15 @@ class Model:
 
     def reserve(self, extra):
         free = [int(i) for i in np.nonzero(self.refs == 0)[0]]
-        asked, granted = 0, []
+        asked, granted, refs = 0, [], self.refs.copy()
         for r, more in enumerate(int(x) for x in extra):
             have, want = self._pages(self.lens[r]), self._pages(self.lens[r] + max(more, 0))
             if more < 0 or want > self.table.shape[1]:
                 self.status |= 2 if more < 0 else 4
+                granted.append(0)
+                continue
+            if more > 0 and self.lens[r] % self.ps and refs[self.table[r, have - 1]] > 1:
+                self.status |= 4                # the positions behind it are another row's
                 granted.append(0)
                 continue
             start, asked = asked, asked + want - have

@@ -100,7 +100,7 @@ struct ReserveParams {
   PageTables t;
   const int32_t* extra;
   int32_t* granted;                              // nullable
-  int *list, *start;                             // pages, R
+  int *list, *start;                             // pages, R; start -1: refused, its last page is shared
 };
 
 __device__ __forceinline__ bool reserve_need(const ReserveParams& p, int r, int& have, int& need, int& len, int& more) {
@@ -115,6 +115,14 @@ __device__ __forceinline__ bool reserve_need(const ReserveParams& p, int r, int&
   return true;
 }
 
+// Whether the row's last page is partly used and other slots name it too (a forked row that was cut inside a shared page, or
+// the row that it was forked from): the positions behind lens are theirs, so the row must not grow into them.
+__device__ __forceinline__ bool reserve_shared(const PageTables& t, int r, int have, int len) {
+  if (len % t.page_size == 0) return false;
+  const int id = t.table[(size_t)r * t.T + have - 1];
+  return id >= 0 && id < t.pages && t.refs[id] > 1;
+}
+
 __global__ void __launch_bounds__(kPgThreads, 1) pages_reserve_kernel(const ReserveParams p) {
   __shared__ int s_warp[32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -126,10 +134,11 @@ __global__ void __launch_bounds__(kPgThreads, 1) pages_reserve_kernel(const Rese
   for (int base = 0; base < p.t.R; base += kPgThreads) {
     const int r = base + tid;
     int have, need = 0, len, more;
-    if (r < p.t.R) reserve_need(p, r, have, need, len, more);
-    const int capped = min(need, cap);
+    bool shared = false;
+    if (r < p.t.R && reserve_need(p, r, have, need, len, more) && more > 0) shared = reserve_shared(p.t, r, have, len);
+    const int capped = shared ? 0 : min(need, cap);
     const int incl = block_scan(capped, s_warp);
-    if (r < p.t.R) p.start[r] = min((long long)total + incl - capped, (long long)cap);
+    if (r < p.t.R) p.start[r] = shared ? -1 : (int)min((long long)total + incl - capped, (long long)cap);
     __syncthreads();
     total = (int)min((long long)total + s_warp[31], (long long)cap);
   }
@@ -138,7 +147,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) pages_reserve_kernel(const Rese
     int have, need, len, more;
     const bool valid = reserve_need(p, r, have, need, len, more);
     const int start = p.start[r];
-    const bool ok = valid && (long long)start + need <= (need > 0 ? found : 0x7fffffff);
+    const bool ok = valid && start >= 0 && (long long)start + need <= (need > 0 ? found : 0x7fffffff);
     if (ok) {
       for (int i = lane; i < need; i += 32) {
         const int id = p.list[start + i];

@@ -77,7 +77,9 @@ def _done(rc, what, check, dev):
 def reserve(page_table, lens, refs, extra, page_size, check=False):
     """Row r grows by extra[r] (>= 0) positions: it gets the pages that it lacks, and lens[r] += extra[r].  A row gets all its
     pages or, where what it and the rows before it need exceeds the free pages (or its table is too short), none, and
-    stays as it is.  Returns granted (R,) int32, 1 or 0."""
+    stays as it is.  So does a row whose last page is partly used and shared (it was cut there by free, or another row was):
+    its next positions belong to the others too.  fork it into an empty row, which gets a page of its own, and free it: that
+    is how a request goes on from a prefix of another one.  Returns granted (R,) int32, 1 or 0."""
     if not check:
         granted = calls().reserve(page_table, lens, refs, extra, page_size)
         if granted is not None:
