@@ -1,0 +1,154 @@
+"""Rows that reserve refused, in steps that do not wait for its outcome: append and compact leave them alone when they are given
+what reserve granted."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from tests.test_gpu_pages import KV, Both
+from tests.test_pages_shared import _held
+from verified_metal_kernels_b200 import _lib, build
+from verified_metal_kernels_b200.kernels import _common, pages_b200
+
+
+def test_refused_before_any_launch():
+    build.build()
+    lib = _lib.lib()
+    pool = (ctypes.c_int64 * 8)(256, 1, 8, 256, 256, 1, 8, 256)
+    src = (ctypes.c_int64 * 6)(256, 2048, 256, 256, 2048, 256)
+    append = lambda granted, tokens=9: lib.vmk_pages_append_granted(pool, src, 8, 64, 256, 4, 256, 256, granted, 2, tokens, None, None)
+    assert append(258) == -1 and append(None, tokens=0) == 0 and append(258, tokens=0) == 0
+    compact = lambda granted, R=2: lib.vmk_pages_compact_granted(pool, 2, 256, R, 4, 256, 256, 8, 64, 256, 256, granted, 4, None, None)
+    assert compact(258) == -1 and compact(256, R=0) == 0
+
+
+def test_modules_refuse_by_their_checks(monkeypatch):
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    i32 = torch.int32
+    table, lens, refs, cu = torch.zeros(2, 4, dtype=i32), torch.zeros(2, dtype=i32), torch.zeros(8, dtype=i32), torch.zeros(2, dtype=i32)
+    pool, k = torch.zeros(8, 2, 16, 8, dtype=torch.float16), torch.zeros(5, 2, 8, dtype=torch.float16)
+    for err, granted in ((TypeError, lens.bool()), (ValueError, lens[:1]), (TypeError, [1, 1])):
+        with pytest.raises(err):
+            pages_b200.append(k, k, pool, pool, table, cu, lens, granted=granted)
+        with pytest.raises(err):
+            pages_b200.compact([pool], table, lens, refs, table, lens, granted=granted)
+
+
+class Steps(Both):
+    def grown(self, extra, pad=0, check=False):
+        """reserve and append, without a look at what was granted in between; the model leaves refused rows alone."""
+        got = pages_b200.reserve(self.table, self.lens, self.refs, self.ints(extra), self.ps)
+        cu = np.concatenate([[0], np.cumsum(extra)]).astype(np.int32)
+        src = [self.rng.standard_normal((int(cu[-1]) + pad, p.shape[2], p.shape[4])).astype(np.float16) for p in self.m.pools]
+        dev = [torch.from_numpy(s).cuda() for s in src]
+        pages_b200.append(dev[0], dev[1], self.pools[0][0], self.pools[1][0], self.table, self.ints(cu), self.lens, granted=got)
+        return self.model_grown(extra, src, cu)
+
+    def model_grown(self, extra, src, cu):
+        want, m = self.m.reserve(extra), self.m
+        for s in np.nonzero(want)[0]:
+            for t in range(cu[s], cu[s + 1]):
+                pos = int(m.lens[s]) - (cu[s + 1] - t)
+                for pool, x in zip(m.pools, src):
+                    pool[0, m.table[s, pos // m.ps], :, pos % m.ps] = x[t]
+        return want
+
+    def closed_up(self, path, count, granted):
+        pages_b200.compact(self.pools, self.table, self.lens, self.refs, self.ints(path), self.ints(count), granted=self.ints(granted))
+        self.m.compact(np.asarray(path), np.where(granted, count, -1))
+
+
+@pytest.mark.gpu
+def test_a_refused_row_keeps_what_it_holds():
+    s = Steps(3, 4, 3, 64, KV, seed=31)
+    s.reserve([60, 64, 30])
+    s.append([60, 64, 30])
+    before = [_held(s.m, r) for r in range(3)]
+    granted = s.grown([8, 1, 8], pad=4)          # no page is left: only row 2 has room
+    assert granted.tolist() == [0, 0, 1]
+    s.same()
+    s.closed_up([[0, 3, -1, -1, -1, -1, -1, -1]] * 3, [2, 2, 2], granted)
+    s.same()
+    assert s.m.lens.tolist() == [60, 64, 32]
+    for r, held in enumerate(before):
+        assert all(np.array_equal(a, b[:len(a)]) for a, b in zip(held, _held(s.m, r)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page_size,rows,pages", [(64, 5, 20), (16, 40, 150), (8, 9, 30)], ids=str)
+def test_random_sequences_with_appended_tokens(page_size, rows, pages):
+    """reserve and append, close up, cut, fork: rows share pages, are cut inside them and run out of pages."""
+    s = Steps(rows, 9, pages, page_size, KV, seed=rows)
+    rng, refused = np.random.default_rng(rows), 0
+    for step in range(30):
+        granted = s.grown(rng.integers(0, 2 * page_size + 1, rows), pad=int(rng.integers(0, 3)))
+        refused += int((granted == 0).sum())
+        s.same()
+        kd = int(rng.integers(1, 7))
+        granted = s.grown(np.full(rows, kd))
+        path, count = np.full((rows, kd), -1), rng.integers(0, kd + 1, rows)
+        for r in range(rows):
+            path[r, :count[r]] = np.sort(rng.permutation(kd)[:count[r]])
+        s.closed_up(path, count, granted)
+        s.same()
+        empty = rng.permutation(rows)[:rows // 3]
+        s.free(np.where(np.isin(np.arange(rows), empty), 0, rng.integers(0, 9 * page_size, rows)))
+        s.fork(rng.integers(-1, rows, len(empty)), empty)
+        s.same()
+    assert refused >= 9                          # the statement alone gives 9, 89 and 16: the steps do meet refusals
+    s.free(np.zeros(rows))
+    s.same()
+    assert (s.m.refs == 0).all()
+
+
+@pytest.mark.gpu
+def test_a_captured_step_replayed_until_the_pages_run_out():
+    s = Steps(4, 8, 14, 64, KV, seed=33)
+    s.reserve([60, 100, 3, 130])
+    s.append([60, 100, 3, 130])
+    extra, cu = s.ints([40, 24, 50, 8]), s.ints([0, 40, 64, 114, 122])
+    src = torch.randn(122, 2, 128, device="cuda").half()
+    path, count = s.ints([[0, 2, 3, -1], [0, -1, -1, -1], [0, 1, 2, 3], [1, 2, -1, -1]]), s.ints([3, 1, 4, 2])
+    rows = []
+
+    def step():
+        granted = pages_b200.reserve(s.table, s.lens, s.refs, extra, 64)
+        pages_b200.append(src, src, s.pools[0][0], s.pools[1][0], s.table, cu, s.lens, granted=granted)
+        pages_b200.compact(s.pools, s.table, s.lens, s.refs, path, count, granted=granted)
+        rows.append(granted)
+
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    host, seen = src.cpu().numpy(), []
+    for _ in range(20):
+        g.replay()
+        want = s.model_grown([40, 24, 50, 8], [host, host], [0, 40, 64, 114, 122])
+        s.m.compact(path.cpu().numpy(), np.where(want, [3, 1, 4, 2], -1))
+        seen.append(rows[0].tolist())
+        assert seen[-1] == want.tolist()
+        s.same()
+    assert seen[0] == [1, 1, 1, 1] and 0 in seen[-1] and len({tuple(x) for x in seen}) > 2
+
+
+@pytest.mark.gpu
+def test_the_compiled_way_takes_granted():
+    calls = _common.calls()
+    got = []
+    for way in (calls.append, pages_b200.append):
+        s = Steps(2, 2, 4, 64, KV, seed=35)
+        s.reserve([70, 9])
+        src, granted = torch.ones(5, 2, 128, dtype=torch.float16, device="cuda"), s.ints([0, 1])
+        args = (src, src, s.pools[0][0], s.pools[1][0], s.table, s.ints([0, 3, 5]), s.lens)
+        if way is calls.append:
+            assert way(*args, granted) is True and calls.append(*args, granted[:1]) is None and calls.append(*args, granted.long()) is None
+            assert calls.compact(s.pools, s.table, s.lens, s.refs, s.ints([[1, -1]] * 2), s.ints([1, 1]), granted) is True
+        else:
+            way(*args, check=True, granted=granted)
+            pages_b200.compact(s.pools, s.table, s.lens, s.refs, s.ints([[1, -1]] * 2), s.ints([1, 1]), check=True, granted=granted)
+        assert s.lens.tolist() == [70, 8]
+        got.append(s.pools)
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    assert _lib.read_status(torch.device("cuda", 0)) == 0

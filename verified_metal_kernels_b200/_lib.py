@@ -50,8 +50,10 @@ SIGNATURES = {
     "vmk_pages_workspace_bytes": (_sz, [_i] * 3),
     "vmk_pages_reserve": (_i, [_vp, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _sz, _vp, _vp]),
     "vmk_pages_append": (_i, [_vp, _vp, _i, _i, _vp, _i, _vp, _vp, _i, _i, _vp, _vp]),
+    "vmk_pages_append_granted": (_i, [_vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _vp, _vp]),
     "vmk_pages_fork": (_i, [_vp, _i, _vp, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _sz, _vp, _vp]),
     "vmk_pages_compact": (_i, [_vp, _i, _vp, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _vp]),
+    "vmk_pages_compact_granted": (_i, [_vp, _i, _vp, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _i, _vp, _vp]),
     "vmk_pages_free": (_i, [_vp, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _vp]),
     "vmk_pages_copy": (_i, [_vp, _i, _i, _i, _vp, _vp, _i, _vp, _vp]),
     "vmk_lse_merge": (_i, [_vp] * 3 + [_i] * 3 + [_vp, _vp]),

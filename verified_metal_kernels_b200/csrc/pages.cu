@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) pages_reserve_kernel(const Rese
 struct FreeParams {
   PageTables t;
   const int32_t* keep;                           // tokens that row r keeps; null: lens - kd + count (after compact)
-  const int32_t* count;
+  const int32_t *count, *granted;                // granted nullable: a row with 0 has no drafts
   int kd;
 };
 
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(256) pages_free_kernel(const FreeParams p) {
     keep = p.keep[r];
     if (keep < 0) { bad = true; keep = len; }    // refused: the row stays as it is
   } else {
-    const int c = p.count[r];
+    const int c = p.granted != nullptr && p.granted[r] == 0 ? -1 : p.count[r];
     keep = c < 0 || len < p.kd ? len : len - p.kd + min(c, p.kd);
   }
   keep = min(keep, len);
@@ -369,7 +369,7 @@ struct AppendSource {
 struct AppendParams {
   PagePools pools;
   AppendSource from[2];
-  const int32_t *table, *cu, *lens;
+  const int32_t *table, *cu, *lens, *granted;    // granted nullable: a row with 0 did not get the positions of its tokens
   int S, T, tokens;
   int32_t* status;
 };
@@ -391,6 +391,7 @@ __global__ void __launch_bounds__(256) pages_append_kernel(const AppendParams p)
     lo += last * step;
     n = min(step, n - last * step);
   }
+  if (p.granted != nullptr && lo < p.S && p.granted[lo] == 0) return;      // lens does not count them: they would fall on older ones
   const int end = p.cu[min(lo + 1, p.S)];
   const long long pos = (long long)p.lens[min(lo, p.S - 1)] - (end - t);
   const long long slot = pos >= 0 ? pos / p.pools.page_size : -1;
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(256) pages_append_kernel(const AppendParams p)
 // ------------------------------------------------------------------------------------------------ compact
 struct CompactParams {
   PagePools pools;
-  const int32_t *table, *lens, *refs, *path, *count;
+  const int32_t *table, *lens, *refs, *path, *count, *granted;
   int R, T, kd, per_row;                         // per_row: 16-byte columns of one position over all pools
   int32_t* status;
 };
@@ -439,7 +440,8 @@ __global__ void __launch_bounds__(256) pages_compact_kernel(const CompactParams 
   int* s_to = s_at + p.kd;
   const int r = blockIdx.x, tid = threadIdx.x;
   pdl_wait();
-  const int len = p.lens[r], n = min(p.count[r], p.kd), base = len - p.kd;
+  const int len = p.lens[r], base = len - p.kd;
+  const int n = p.granted != nullptr && p.granted[r] == 0 ? -1 : min(p.count[r], p.kd);
   const int ps = p.pools.page_size;
   for (int j = tid; j < p.kd; j += 256) {
     int from = -1, to = -1;
@@ -585,6 +587,12 @@ extern "C" int vmk_pages_copy(const int64_t* pools, int n_pools, int pages, int 
 extern "C" int vmk_pages_append(const int64_t* pools, const int64_t* sources, int pages, int page_size, const int32_t* page_table,
                                 int table_stride, const int32_t* cu, const int32_t* lens, int S, int tokens, int32_t* status,
                                 void* stream) {
+  return vmk_pages_append_granted(pools, sources, pages, page_size, page_table, table_stride, cu, lens, nullptr, S, tokens, status, stream);
+}
+
+extern "C" int vmk_pages_append_granted(const int64_t* pools, const int64_t* sources, int pages, int page_size,
+                                        const int32_t* page_table, int table_stride, const int32_t* cu, const int32_t* lens,
+                                        const int32_t* granted, int S, int tokens, int32_t* status, void* stream) {
   AppendParams p;
   memset(&p, 0, sizeof(p));
   const int rc = read_pools(p.pools, pools, 2, pages, page_size, 2);
@@ -592,7 +600,8 @@ extern "C" int vmk_pages_append(const int64_t* pools, const int64_t* sources, in
   if (sources == nullptr || S < 0 || tokens < 0 || table_stride <= 0) return VMK_E_BADARG;
   if (p.pools.pool[0].layers != 1 || p.pools.pool[1].layers != 1) return VMK_E_UNSUPPORTED;
   if (S == 0 || tokens == 0) return VMK_OK;
-  if (pg_bad(page_table, 4) || pg_bad(cu, 4) || pg_bad(lens, 4) || (status && pg_bad(status, 4))) return VMK_E_BADARG;
+  if (pg_bad(page_table, 4) || pg_bad(cu, 4) || pg_bad(lens, 4) || (granted && pg_bad(granted, 4)) || (status && pg_bad(status, 4)))
+    return VMK_E_BADARG;
   if (tokens > 0x7fffffff / 32 - 256) return VMK_E_TOO_LARGE;
   for (int i = 0; i < 2; ++i) {
     const int64_t* d = sources + 3 * i;
@@ -602,6 +611,7 @@ extern "C" int vmk_pages_append(const int64_t* pools, const int64_t* sources, in
   p.table = page_table;
   p.cu = cu;
   p.lens = lens;
+  p.granted = granted;
   p.S = S;
   p.T = table_stride;
   p.tokens = tokens;
@@ -678,6 +688,13 @@ extern "C" int vmk_pages_fork(const int64_t* pools, int n_pools, int32_t* page_t
 extern "C" int vmk_pages_compact(const int64_t* pools, int n_pools, int32_t* page_table, int R, int table_stride, int32_t* lens,
                                  int32_t* refs, int pages, int page_size, const int32_t* path, const int32_t* count, int kd,
                                  int32_t* status, void* stream) {
+  return vmk_pages_compact_granted(pools, n_pools, page_table, R, table_stride, lens, refs, pages, page_size, path, count, nullptr, kd,
+                                   status, stream);
+}
+
+extern "C" int vmk_pages_compact_granted(const int64_t* pools, int n_pools, int32_t* page_table, int R, int table_stride,
+                                         int32_t* lens, int32_t* refs, int pages, int page_size, const int32_t* path,
+                                         const int32_t* count, const int32_t* granted, int kd, int32_t* status, void* stream) {
   CompactParams p;
   FreeParams f;
   memset(&p, 0, sizeof(p));
@@ -688,12 +705,13 @@ extern "C" int vmk_pages_compact(const int64_t* pools, int n_pools, int32_t* pag
   if (kd <= 0) return VMK_E_BADARG;
   if (kd > VMK_SPEC_MAX_DRAFTS) return VMK_E_UNSUPPORTED;
   if (R == 0) return VMK_OK;
-  if (pg_bad(path, 4) || pg_bad(count, 4)) return VMK_E_BADARG;
+  if (pg_bad(path, 4) || pg_bad(count, 4) || (granted && pg_bad(granted, 4))) return VMK_E_BADARG;
   p.table = page_table;
   p.lens = lens;
   p.refs = refs;
   p.path = path;
   p.count = count;
+  p.granted = f.granted = granted;
   p.R = R;
   p.T = table_stride;
   p.kd = kd;

@@ -29,9 +29,9 @@ struct Entries {
   decltype(&vmk_accept) accept;
   decltype(&vmk_pages_workspace_bytes) pages_ws;
   decltype(&vmk_pages_reserve) reserve;
-  decltype(&vmk_pages_append) append;
+  decltype(&vmk_pages_append_granted) append;
   decltype(&vmk_pages_fork) fork;
-  decltype(&vmk_pages_compact) compact;
+  decltype(&vmk_pages_compact_granted) compact;
   decltype(&vmk_pages_free) free;
   decltype(&vmk_pages_copy) copy;
 } g_entry = {};
@@ -248,13 +248,23 @@ PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// append(k, v, k_pages, v_pages, page_table, cu, lens)
+// What reserve granted, where it is given: false if that is no int32 tensor of R entries.
+bool granted_of(int32_t*& p, const Call& c, PyObject* o, int R) {
+  p = nullptr;
+  if (o == Py_None) return true;
+  const at::Tensor* t = ints(o, c, 1, R);
+  if (t) p = ip(t);
+  return t != nullptr;
+}
+
+// append(k, v, k_pages, v_pages, page_table, cu, lens, granted=None)
 PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Call c;
     State s;
     Pools p;
-    if (n != 7 || !begin(c) || !state(s, c, a[4], a[6], nullptr)) return none();
+    int32_t* granted;
+    if ((n != 7 && n != 8) || !begin(c) || !state(s, c, a[4], a[6], nullptr) || !granted_of(granted, c, n == 8 ? a[7] : Py_None, s.R)) return none();
     const at::Tensor* cu = ints(a[5], c, 1);
     if (!cu || cu->size(0) < 1 || cu->size(0) - 1 > s.R) return none();
     int64_t src[6], tokens = -1;
@@ -269,8 +279,8 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       src[3 * i + 1] = by_token;
       src[3 * i + 2] = by_head;
     }
-    const int rc = g_entry.append(p.d, src, (int)p.pages, (int)p.page_size, ip(s.table), s.T, ip(cu), ip(s.lens), (int)cu->size(0) - 1, (int)tokens, c.status,
-                                  c.stream);
+    const int rc = g_entry.append(p.d, src, (int)p.pages, (int)p.page_size, ip(s.table), s.T, ip(cu), ip(s.lens), granted, (int)cu->size(0) - 1, (int)tokens,
+                                  c.status, c.stream);
     return rc == VMK_OK ? yes() : none();
   });
 }
@@ -292,17 +302,19 @@ PyObject* fork_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// compact(pools, page_table, lens, refs, path, count)
+// compact(pools, page_table, lens, refs, path, count, granted=None)
 PyObject* compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Call c;
     State s;
     Pools p;
-    if (n != 6 || !begin(c) || !state(s, c, a[1], a[2], a[3]) || !pools(p, c, a[0]) || s.refs->size(0) != p.pages) return none();
+    int32_t* granted;
+    if ((n != 6 && n != 7) || !begin(c) || !state(s, c, a[1], a[2], a[3]) || !pools(p, c, a[0]) || s.refs->size(0) != p.pages || !granted_of(granted, c, n == 7 ? a[6] : Py_None, s.R))
+      return none();
     const at::Tensor *path = ints(a[4], c, 2, s.R), *count = ints(a[5], c, 1, s.R);
     if (!path || !count || !fits(path->size(1))) return none();
     const int rc = g_entry.compact(p.d, p.n, ip(s.table), s.R, s.T, ip(s.lens), ip(s.refs), (int)p.pages, (int)p.page_size, ip(path), ip(count),
-                                   (int)path->size(1), c.status, c.stream);
+                                   granted, (int)path->size(1), c.status, c.stream);
     return rc == VMK_OK ? yes() : none();
   });
 }

@@ -8,7 +8,7 @@ import torch
 from .. import _lib
 
 _ENTRIES = ("vmk_prompt_workspace_bytes", "vmk_prompt", "vmk_prompt_paged", "vmk_accept", "vmk_pages_workspace_bytes",
-            "vmk_pages_reserve", "vmk_pages_append", "vmk_pages_fork", "vmk_pages_compact", "vmk_pages_free", "vmk_pages_copy")
+            "vmk_pages_reserve", "vmk_pages_append_granted", "vmk_pages_fork", "vmk_pages_compact_granted", "vmk_pages_free", "vmk_pages_copy")
 _calls = None
 
 

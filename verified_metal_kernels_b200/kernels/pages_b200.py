@@ -99,14 +99,20 @@ def reserve(page_table, lens, refs, extra, page_size, check=False):
     return granted
 
 
-def append(k, v, k_pages, v_pages, page_table, cu, lens, check=False):
+def append(k, v, k_pages, v_pages, page_table, cu, lens, check=False, granted=None):
     """Writes packed tokens into their pages: k, v (tokens,heads,width) -- views are fine, the innermost axis contiguous --
     and tokens [cu[s], cu[s+1]) of row s become its last positions: lens[s] counts them already (reserve before append).
     k_pages, v_pages (pages,heads,page_size,width), or (pages,page_size,width) for one head; k and v may differ in
-    heads and width (dsa: latent rows and index keys).  Tokens outside [cu[0], cu[-1]) are not written."""
-    if not check and calls().append(k, v, k_pages, v_pages, page_table, cu, lens):
+    heads and width (dsa: latent rows and index keys).  Tokens outside [cu[0], cu[-1]) are not written.
+
+    granted (R,) int32, as reserve returns it: the tokens of a row with 0 are not written.  A step that does not wait for
+    the outcome of reserve passes it on here and to compact: lens of a refused row does not count its tokens, which would
+    take the place of the row's last ones."""
+    if not check and calls().append(k, v, k_pages, v_pages, page_table, cu, lens, granted):
         return
     R, T, dev = _state(page_table, lens, None)
+    if granted is not None:
+        need_on(granted, "granted", torch.int32, (R,), dev)
     need(cu, "cu", torch.int32, dims=1)
     S = cu.shape[0] - 1
     if S < 0 or S > R:
@@ -134,11 +140,11 @@ def append(k, v, k_pages, v_pages, page_table, cu, lens, check=False):
     lib = _lib.lib()
     if elsewhere(dev):
         with torch.cuda.device(dev):
-            return append(k, v, k_pages, v_pages, page_table, cu, lens, check)
+            return append(k, v, k_pages, v_pages, page_table, cu, lens, check, granted)
     stream, status = handles(dev)
-    rc = lib.vmk_pages_append(pools, struct.pack("6q", *src), pages, page_size, page_table.data_ptr(), T, cu.data_ptr(), lens.data_ptr(), S,
-                              tokens, status, stream)
-    _done(rc, "vmk_pages_append", check, dev)
+    rc = lib.vmk_pages_append_granted(pools, struct.pack("6q", *src), pages, page_size, page_table.data_ptr(), T, cu.data_ptr(),
+                                      lens.data_ptr(), _lib.ptr(granted), S, tokens, status, stream)
+    _done(rc, "vmk_pages_append_granted", check, dev)
 
 
 def fork(pools, page_table, lens, refs, parents, children, check=False):
@@ -166,11 +172,12 @@ def fork(pools, page_table, lens, refs, parents, children, check=False):
     _done(rc, "vmk_pages_fork", check, dev)
 
 
-def compact(pools, page_table, lens, refs, path, count, check=False):
+def compact(pools, page_table, lens, refs, path, count, check=False, granted=None):
     """After kd drafts at the end of each row were verified: the accepted ones, path (R,kd) int32 and count (R,) int32 as
     accept_b200.kernel gives them, close up behind the positions before the drafts, lens[r] becomes lens[r] - kd +
-    count[r], and pages behind that are given back.  count[r] < 0: the row stays as it is."""
-    if not check and calls().compact(pools, page_table, lens, refs, path, count):
+    count[r], and pages behind that are given back.  count[r] < 0: the row stays as it is, and so does a row with 0 in
+    granted (R,) int32 (see append): it got no place for its drafts."""
+    if not check and calls().compact(pools, page_table, lens, refs, path, count, granted):
         return
     R, T, dev = _state(page_table, lens, refs)
     desc, pages, page_size = _pools(pools, dev)
@@ -179,14 +186,16 @@ def compact(pools, page_table, lens, refs, path, count, check=False):
     kd = path.shape[1]
     need_on(path, "path", torch.int32, (R, kd), dev)
     need_on(count, "count", torch.int32, (R,), dev)
+    if granted is not None:
+        need_on(granted, "granted", torch.int32, (R,), dev)
     lib = _lib.lib()
     if elsewhere(dev):
         with torch.cuda.device(dev):
-            return compact(pools, page_table, lens, refs, path, count, check)
+            return compact(pools, page_table, lens, refs, path, count, check, granted)
     stream, status = handles(dev)
-    rc = lib.vmk_pages_compact(desc, len(pools), page_table.data_ptr(), R, T, lens.data_ptr(), refs.data_ptr(), pages, page_size, path.data_ptr(),
-                               count.data_ptr(), kd, status, stream)
-    _done(rc, "vmk_pages_compact", check, dev)
+    rc = lib.vmk_pages_compact_granted(desc, len(pools), page_table.data_ptr(), R, T, lens.data_ptr(), refs.data_ptr(), pages, page_size,
+                                       path.data_ptr(), count.data_ptr(), _lib.ptr(granted), kd, status, stream)
+    _done(rc, "vmk_pages_compact_granted", check, dev)
 
 
 def free(page_table, lens, refs, keep, page_size, check=False):
