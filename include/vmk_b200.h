@@ -332,8 +332,9 @@ VMK_API int vmk_accept(const void* target_probs, const void* draft_probs, const 
  *   that is not empty, is named twice (the first has it) or out of range is refused (status bit 1).
  * vmk_pages_compact: after a verification of kd drafts at the end of each row: the accepted ones, path[r][0 .. count[r])
  *   ascending (as vmk_accept gives them), close up behind the rest, lens[r] becomes lens[r] - kd + count[r], and pages
- *   behind that are given back.  count[r] < 0: the row stays as it is.  Drafts in a page that other rows share are not
- *   moved (status bit 2); a path that does not ascend is not followed where it does not (status bit 1).  kd <= 128.
+ *   behind that are given back.  count[r] < 0: the row stays as it is.  So does, length and pages, a row one of whose
+ *   entries cannot move: into a page that other rows share (status bit 2), or along a path that does not ascend (status bit
+ *   1); it is known by its length, which still counts the kd drafts.  kd <= 128.  lens holds no length while the call runs.
  * vmk_pages_free: row r keeps its first keep[r] >= 0 positions and gives back (refs - 1) the pages behind them; its freed
  *   slots become -1.
  * vmk_pages_copy: page src[i] -> page dst[i] in every pool, i < n; a page is not both among src and dst, nor twice in dst.

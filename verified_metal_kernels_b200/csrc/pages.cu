@@ -177,7 +177,12 @@ __global__ void __launch_bounds__(256) pages_free_kernel(const FreeParams p) {
   const int r = (blockIdx.x * 256 + threadIdx.x) >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   if (r >= p.t.R) return;
-  const int len = max(p.t.lens[r], 0);
+  const int marked = p.t.lens[r], len = max(marked, 0);
+  __syncwarp();                                  // every lane has read lens before lane 0 writes it
+  if (p.keep == nullptr && marked < 0) {         // compact refused the row: length and pages as they were
+    if (lane == 0) p.t.lens[r] = ~marked;
+    return;
+  }
   int keep;
   bool bad = false;
   if (p.keep != nullptr) {
@@ -426,7 +431,8 @@ __global__ void __launch_bounds__(256) pages_append_kernel(const AppendParams p)
 // ------------------------------------------------------------------------------------------------ compact
 struct CompactParams {
   PagePools pools;
-  const int32_t *table, *lens, *refs, *path, *count, *granted;
+  int32_t* lens;
+  const int32_t *table, *refs, *path, *count, *granted;
   int R, T, kd, per_row;                         // per_row: 16-byte columns of one position over all pools
   int32_t* status;
 };
@@ -434,15 +440,21 @@ struct CompactParams {
 // A thread owns one 16-byte column of a row's positions and moves it down the path: entry j goes from base + path[j] to
 // base + j with path[j] >= j ascending, so a source is never a destination of an earlier entry, and reads of eight
 // entries may go before their writes.
+//
+// A row moves as a whole or not at all: where one of its entries cannot move (its new place is in a page that others share, the
+// path does not ascend) nothing is written and the row stays as it is, or its positions would hold other drafts than the
+// accepted ones.  Every CTA of the row comes to that by itself; its first one tells the free that follows by the one word that
+// both see, lens, which it turns negative (~lens) until then.  A CTA that reads lens after that knows the same.
 __global__ void __launch_bounds__(256) pages_compact_kernel(const CompactParams p) {
   extern __shared__ int s_at[];                  // [kd] source page * page_size + row, [kd] destination; -1: nothing to move
   int* s_from = s_at;
   int* s_to = s_at + p.kd;
   const int r = blockIdx.x, tid = threadIdx.x;
   pdl_wait();
-  const int len = p.lens[r], base = len - p.kd;
+  const int len = *const_cast<const volatile int32_t*>(p.lens + r), base = len - p.kd;
   const int n = p.granted != nullptr && p.granted[r] == 0 ? -1 : min(p.count[r], p.kd);
   const int ps = p.pools.page_size;
+  bool refused = false;
   for (int j = tid; j < p.kd; j += 256) {
     int from = -1, to = -1;
     bool bad = false, shared = false;
@@ -467,11 +479,13 @@ __global__ void __launch_bounds__(256) pages_compact_kernel(const CompactParams 
     }
     if (blockIdx.y == 0 && bad) report(p.status, kStatusBadIndex);
     if (blockIdx.y == 0 && shared) report(p.status, kStatusPages);
+    refused |= bad || shared;
     s_at[2 * p.kd + j] = from;
     s_at[3 * p.kd + j] = to;
   }
-  __syncthreads();
-  if (n <= 0) return;
+  refused = __syncthreads_or(refused);
+  if (blockIdx.y == 0 && tid == 0 && (refused || len < 0)) p.lens[r] = ~max(len, 0);      // (len < 0: no length, it becomes 0)
+  if (n <= 0 || refused) return;
   for (int c0 = blockIdx.y * 256 + tid; c0 < p.per_row; c0 += gridDim.y * 256) {
     int c = c0, i = 0;
     for (;; ++i) {

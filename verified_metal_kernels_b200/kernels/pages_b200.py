@@ -176,7 +176,10 @@ def compact(pools, page_table, lens, refs, path, count, check=False, granted=Non
     """After kd drafts at the end of each row were verified: the accepted ones, path (R,kd) int32 and count (R,) int32 as
     accept_b200.kernel gives them, close up behind the positions before the drafts, lens[r] becomes lens[r] - kd +
     count[r], and pages behind that are given back.  count[r] < 0: the row stays as it is, and so does a row with 0 in
-    granted (R,) int32 (see append): it got no place for its drafts."""
+    granted (R,) int32 (see append): it got no place for its drafts.
+
+    A row moves as a whole or not at all: where an entry would move into a page that other rows share, or its path does not
+    ascend, the row keeps its length and its pages (and the call reports it)."""
     if not check and calls().compact(pools, page_table, lens, refs, path, count, granted):
         return
     R, T, dev = _state(page_table, lens, refs)
