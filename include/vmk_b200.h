@@ -326,7 +326,9 @@ VMK_API int vmk_accept(const void* target_probs, const void* draft_probs, const 
  * vmk_pages_append_granted, vmk_pages_compact_granted: the same with what reserve granted (R, nullable): the tokens of a
  *   row with 0 are not written, and the row has no drafts to compact.  lens of such a row does not count its tokens:
  *   without `granted` they would take the place of its last ones, and compact would take those for drafts.  So a step that does
- *   not wait for the outcome of reserve (a captured one, say) passes it on.
+ *   not wait for the outcome of reserve (a captured one, say) passes it on.  refs (pages, nullable): a token whose page other
+ *   slots name as well is not written (status bit 2); after reserve there is none, unless a row was forked between the two
+ *   calls.
  * vmk_pages_fork: entry f makes row children[f] (of length 0) a copy of row parents[f]: full pages are shared (refs + 1), of
  *   a last page that is not full a new page gets the used rows, in every pool.  parents[f] < 0: nothing to do.  A child
  *   that is not empty, is named twice (the first has it) or out of range is refused (status bit 1).
@@ -348,7 +350,8 @@ VMK_API int vmk_pages_append(const int64_t* pools, const int64_t* sources, int p
                              int tokens, int32_t* status, void* stream);
 VMK_API int vmk_pages_append_granted(const int64_t* pools, const int64_t* sources, int pages, int page_size,
                                      const int32_t* page_table, int table_stride, const int32_t* cu, const int32_t* lens,
-                                     const int32_t* granted, int S, int tokens, int32_t* status, void* stream);
+                                     const int32_t* refs, const int32_t* granted, int S, int tokens, int32_t* status,
+                                     void* stream);
 VMK_API int vmk_pages_fork(const int64_t* pools, int n_pools, int32_t* page_table, int R, int table_stride, int32_t* lens,
                            int32_t* refs, int pages, int page_size, const int32_t* parents, const int32_t* children, int F,
                            void* ws, size_t ws_bytes, int32_t* status, void* stream);

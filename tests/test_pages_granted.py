@@ -17,7 +17,7 @@ def test_refused_before_any_launch():
     lib = _lib.lib()
     pool = (ctypes.c_int64 * 8)(256, 1, 8, 256, 256, 1, 8, 256)
     src = (ctypes.c_int64 * 6)(256, 2048, 256, 256, 2048, 256)
-    append = lambda granted, tokens=9: lib.vmk_pages_append_granted(pool, src, 8, 64, 256, 4, 256, 256, granted, 2, tokens, None, None)
+    append = lambda granted, tokens=9: lib.vmk_pages_append_granted(pool, src, 8, 64, 256, 4, 256, 256, None, granted, 2, tokens, None, None)
     assert append(258) == -1 and append(None, tokens=0) == 0 and append(258, tokens=0) == 0
     compact = lambda granted, R=2: lib.vmk_pages_compact_granted(pool, 2, 256, R, 4, 256, 256, 8, 64, 256, 256, granted, 4, None, None)
     assert compact(258) == -1 and compact(256, R=0) == 0

@@ -6,6 +6,8 @@ import torch
 
 from tests._pages_model import Model
 from tests.test_gpu_pages import KV, Both
+from verified_metal_kernels_b200 import _lib
+from verified_metal_kernels_b200.kernels import _common, pages_b200
 
 
 def _model(rows, width, pages, page_size):
@@ -92,3 +94,39 @@ def test_both_rows_cut_in_the_same_page_and_a_row_that_asks_for_nothing():
     assert s.m.lens.tolist() == [70, 127, 5, 0]
     s.reserve([0, 0, 0, 0])                     # no growth is always granted
     s.same()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("compiled", [True, False], ids=["compiled", "module"])
+def test_append_with_the_counts_writes_no_shared_page(compiled):
+    """A row forked between its reserve and its append: the positions that are still to be written are both rows'."""
+    s = Both(3, 4, 12, 64, KV, seed=23)
+    s.reserve([60, 10, 0])
+    s.append([60, 10])
+    s.reserve([68, 5, 0])                        # to 128: two full pages, which the fork shares
+    s.fork([0], [2])
+    s.same()
+    before = [p.clone() for p in s.pools]
+    src = torch.ones(73, 2, 128, dtype=torch.float16, device="cuda")
+    args = (src, src, s.pools[0][0], s.pools[1][0], s.table, s.ints([0, 68, 73]), s.lens)
+    if compiled:
+        assert _common.calls().append(*args, None, s.refs) is True and _common.calls().append(*args, None, s.refs[:-1].contiguous()) is None
+    else:
+        with pytest.raises(_lib.VmkDeviceStatusError) as e:
+            pages_b200.append(*args, check=True, refs=s.refs)
+        assert e.value.status == 4
+    host = src[68:].cpu().numpy()
+    s.m.append([host, host], [0, 0, 5])          # row 1's, and nothing else
+    s.m.status = 4 if compiled else 0
+    s.same()
+    assert not torch.equal(before[0], s.pools[0])
+
+
+def test_append_refuses_wrong_counts(monkeypatch):
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    i32 = torch.int32
+    table, lens, cu = torch.zeros(2, 4, dtype=i32), torch.zeros(2, dtype=i32), torch.zeros(2, dtype=i32)
+    pool, k = torch.zeros(8, 2, 16, 8, dtype=torch.float16), torch.zeros(5, 2, 8, dtype=torch.float16)
+    for err, refs in ((ValueError, torch.zeros(7, dtype=i32)), (TypeError, torch.zeros(8)), (TypeError, [0] * 8)):
+        with pytest.raises(err):
+            pages_b200.append(k, k, pool, pool, table, cu, lens, refs=refs)

@@ -50,7 +50,7 @@ SIGNATURES = {
     "vmk_pages_workspace_bytes": (_sz, [_i] * 3),
     "vmk_pages_reserve": (_i, [_vp, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _sz, _vp, _vp]),
     "vmk_pages_append": (_i, [_vp, _vp, _i, _i, _vp, _i, _vp, _vp, _i, _i, _vp, _vp]),
-    "vmk_pages_append_granted": (_i, [_vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _vp, _vp]),
+    "vmk_pages_append_granted": (_i, [_vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp]),
     "vmk_pages_fork": (_i, [_vp, _i, _vp, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _sz, _vp, _vp]),
     "vmk_pages_compact": (_i, [_vp, _i, _vp, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _vp]),
     "vmk_pages_compact_granted": (_i, [_vp, _i, _vp, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _i, _vp, _vp]),

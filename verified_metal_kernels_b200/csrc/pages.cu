@@ -374,7 +374,8 @@ struct AppendSource {
 struct AppendParams {
   PagePools pools;
   AppendSource from[2];
-  const int32_t *table, *cu, *lens, *granted;    // granted nullable: a row with 0 did not get the positions of its tokens
+  const int32_t *table, *cu, *lens;
+  const int32_t *refs, *granted;                 // both nullable; granted 0: the row did not get the positions of its tokens
   int S, T, tokens;
   int32_t* status;
 };
@@ -403,6 +404,10 @@ __global__ void __launch_bounds__(256) pages_append_kernel(const AppendParams p)
   const int id = lo < p.S && slot >= 0 && slot < p.T ? p.table[(size_t)lo * p.T + slot] : -1;
   if (id < 0 || id >= p.pools.pages) {
     if (lane == 0) report(p.status, kStatusBadIndex);
+    return;
+  }
+  if (p.refs != nullptr && p.refs[id] > 1) {     // other rows' positions too
+    if (lane == 0) report(p.status, kStatusPages);
     return;
   }
   const int row = (int)(pos - slot * p.pools.page_size);
@@ -601,12 +606,14 @@ extern "C" int vmk_pages_copy(const int64_t* pools, int n_pools, int pages, int 
 extern "C" int vmk_pages_append(const int64_t* pools, const int64_t* sources, int pages, int page_size, const int32_t* page_table,
                                 int table_stride, const int32_t* cu, const int32_t* lens, int S, int tokens, int32_t* status,
                                 void* stream) {
-  return vmk_pages_append_granted(pools, sources, pages, page_size, page_table, table_stride, cu, lens, nullptr, S, tokens, status, stream);
+  return vmk_pages_append_granted(pools, sources, pages, page_size, page_table, table_stride, cu, lens, nullptr, nullptr, S, tokens,
+                                  status, stream);
 }
 
 extern "C" int vmk_pages_append_granted(const int64_t* pools, const int64_t* sources, int pages, int page_size,
                                         const int32_t* page_table, int table_stride, const int32_t* cu, const int32_t* lens,
-                                        const int32_t* granted, int S, int tokens, int32_t* status, void* stream) {
+                                        const int32_t* refs, const int32_t* granted, int S, int tokens, int32_t* status,
+                                        void* stream) {
   AppendParams p;
   memset(&p, 0, sizeof(p));
   const int rc = read_pools(p.pools, pools, 2, pages, page_size, 2);
@@ -614,7 +621,8 @@ extern "C" int vmk_pages_append_granted(const int64_t* pools, const int64_t* sou
   if (sources == nullptr || S < 0 || tokens < 0 || table_stride <= 0) return VMK_E_BADARG;
   if (p.pools.pool[0].layers != 1 || p.pools.pool[1].layers != 1) return VMK_E_UNSUPPORTED;
   if (S == 0 || tokens == 0) return VMK_OK;
-  if (pg_bad(page_table, 4) || pg_bad(cu, 4) || pg_bad(lens, 4) || (granted && pg_bad(granted, 4)) || (status && pg_bad(status, 4)))
+  if (pg_bad(page_table, 4) || pg_bad(cu, 4) || pg_bad(lens, 4) || (refs && pg_bad(refs, 4)) || (granted && pg_bad(granted, 4)) ||
+      (status && pg_bad(status, 4)))
     return VMK_E_BADARG;
   if (tokens > 0x7fffffff / 32 - 256) return VMK_E_TOO_LARGE;
   for (int i = 0; i < 2; ++i) {
@@ -625,6 +633,7 @@ extern "C" int vmk_pages_append_granted(const int64_t* pools, const int64_t* sou
   p.table = page_table;
   p.cu = cu;
   p.lens = lens;
+  p.refs = refs;
   p.granted = granted;
   p.S = S;
   p.T = table_stride;

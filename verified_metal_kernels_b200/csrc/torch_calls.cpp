@@ -248,23 +248,23 @@ PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// What reserve granted, where it is given: false if that is no int32 tensor of R entries.
-bool granted_of(int32_t*& p, const Call& c, PyObject* o, int R) {
+// An int32 tensor of n entries or None: false if it is neither.
+bool ints_or_none(int32_t*& p, const Call& c, PyObject* o, int64_t n) {
   p = nullptr;
   if (o == Py_None) return true;
-  const at::Tensor* t = ints(o, c, 1, R);
+  const at::Tensor* t = ints(o, c, 1, n);
   if (t) p = ip(t);
   return t != nullptr;
 }
 
-// append(k, v, k_pages, v_pages, page_table, cu, lens, granted=None)
+// append(k, v, k_pages, v_pages, page_table, cu, lens, granted=None, refs=None)
 PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Call c;
     State s;
     Pools p;
-    int32_t* granted;
-    if ((n != 7 && n != 8) || !begin(c) || !state(s, c, a[4], a[6], nullptr) || !granted_of(granted, c, n == 8 ? a[7] : Py_None, s.R)) return none();
+    int32_t *granted, *refs;
+    if (n < 7 || n > 9 || !begin(c) || !state(s, c, a[4], a[6], nullptr) || !ints_or_none(granted, c, n > 7 ? a[7] : Py_None, s.R)) return none();
     const at::Tensor* cu = ints(a[5], c, 1);
     if (!cu || cu->size(0) < 1 || cu->size(0) - 1 > s.R) return none();
     int64_t src[6], tokens = -1;
@@ -279,7 +279,8 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       src[3 * i + 1] = by_token;
       src[3 * i + 2] = by_head;
     }
-    const int rc = g_entry.append(p.d, src, (int)p.pages, (int)p.page_size, ip(s.table), s.T, ip(cu), ip(s.lens), granted, (int)cu->size(0) - 1, (int)tokens,
+    if (!ints_or_none(refs, c, n > 8 ? a[8] : Py_None, p.pages)) return none();
+    const int rc = g_entry.append(p.d, src, (int)p.pages, (int)p.page_size, ip(s.table), s.T, ip(cu), ip(s.lens), refs, granted, (int)cu->size(0) - 1, (int)tokens,
                                   c.status, c.stream);
     return rc == VMK_OK ? yes() : none();
   });
@@ -309,7 +310,7 @@ PyObject* compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
     State s;
     Pools p;
     int32_t* granted;
-    if ((n != 6 && n != 7) || !begin(c) || !state(s, c, a[1], a[2], a[3]) || !pools(p, c, a[0]) || s.refs->size(0) != p.pages || !granted_of(granted, c, n == 7 ? a[6] : Py_None, s.R))
+    if ((n != 6 && n != 7) || !begin(c) || !state(s, c, a[1], a[2], a[3]) || !pools(p, c, a[0]) || s.refs->size(0) != p.pages || !ints_or_none(granted, c, n == 7 ? a[6] : Py_None, s.R))
       return none();
     const at::Tensor *path = ints(a[4], c, 2, s.R), *count = ints(a[5], c, 1, s.R);
     if (!path || !count || !fits(path->size(1))) return none();

@@ -99,7 +99,7 @@ def reserve(page_table, lens, refs, extra, page_size, check=False):
     return granted
 
 
-def append(k, v, k_pages, v_pages, page_table, cu, lens, check=False, granted=None):
+def append(k, v, k_pages, v_pages, page_table, cu, lens, check=False, granted=None, refs=None):
     """Writes packed tokens into their pages: k, v (tokens,heads,width) -- views are fine, the innermost axis contiguous --
     and tokens [cu[s], cu[s+1]) of row s become its last positions: lens[s] counts them already (reserve before append).
     k_pages, v_pages (pages,heads,page_size,width), or (pages,page_size,width) for one head; k and v may differ in
@@ -107,8 +107,9 @@ def append(k, v, k_pages, v_pages, page_table, cu, lens, check=False, granted=No
 
     granted (R,) int32, as reserve returns it: the tokens of a row with 0 are not written.  A step that does not wait for
     the outcome of reserve passes it on here and to compact: lens of a refused row does not count its tokens, which would
-    take the place of the row's last ones."""
-    if not check and calls().append(k, v, k_pages, v_pages, page_table, cu, lens, granted):
+    take the place of the row's last ones.  refs (pages,) int32: a token whose page other rows share is not written (and
+    reported); after reserve there is none, unless a row was forked between the two calls."""
+    if not check and calls().append(k, v, k_pages, v_pages, page_table, cu, lens, granted, refs):
         return
     R, T, dev = _state(page_table, lens, None)
     if granted is not None:
@@ -118,6 +119,8 @@ def append(k, v, k_pages, v_pages, page_table, cu, lens, check=False, granted=No
     if S < 0 or S > R:
         raise ValueError(f"cu: expected 1 to {R + 1} entries, got {cu.shape[0]}")
     pools, pages, page_size = _pools([k_pages, v_pages], dev)
+    if refs is not None:
+        need_on(refs, "refs", torch.int32, (pages,), dev)
     if k_pages.dim() == 5 or v_pages.dim() == 5:
         raise ValueError("k_pages, v_pages: expected the pools of one layer")
     tokens, src = len(k) if isinstance(k, torch.Tensor) and k.dim() else 0, []
@@ -140,10 +143,11 @@ def append(k, v, k_pages, v_pages, page_table, cu, lens, check=False, granted=No
     lib = _lib.lib()
     if elsewhere(dev):
         with torch.cuda.device(dev):
-            return append(k, v, k_pages, v_pages, page_table, cu, lens, check, granted)
+            return append(k, v, k_pages, v_pages, page_table, cu, lens, check, granted, refs)
     stream, status = handles(dev)
     rc = lib.vmk_pages_append_granted(pools, struct.pack("6q", *src), pages, page_size, page_table.data_ptr(), T, cu.data_ptr(),
-                                      lens.data_ptr(), _lib.ptr(granted), S, tokens, status, stream)
+                                      lens.data_ptr(), _lib.ptr(refs), _lib.ptr(granted), S, tokens, status,
+                                      stream)
     _done(rc, "vmk_pages_append_granted", check, dev)
 
 
