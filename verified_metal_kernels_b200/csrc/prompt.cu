@@ -1085,8 +1085,10 @@ __global__ void __launch_bounds__(256, K > 2 ? 2 : 6) prompt_merge_kernel(const 
   }
   m = warp_max(m);
   float w[2], l = 0.f;
+  uint32_t seen[2];                                      // shares in which the row saw a key: all of these are read
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
+    seen[s] = __ballot_sync(0xffffffffu, ml[s].x != -INFINITY);
     w[s] = ml[s].x == -INFINITY ? 0.f : pm_exp2(ml[s].x - m);
     l += ml[s].x == -INFINITY && ml[s].y == 0.f ? 0.f : w[s] * ml[s].y;
   }
@@ -1101,10 +1103,11 @@ __global__ void __launch_bounds__(256, K > 2 ? 2 : 6) prompt_merge_kernel(const 
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         wi[k][s] = __shfl_sync(0xffffffffu, w[s], (i + k) & 31);
-        if (i + k >= parts) wi[k][s] = 0.f;
+        const bool read = i + k < parts && (seen[s] >> (i + k) & 1u) != 0u;
         v[k][s] = make_float4(0.f, 0.f, 0.f, 0.f);
-        // a share that this row sees nothing of may not have been written
-        if (wi[k][s] != 0.f) v[k][s] = *reinterpret_cast<const float4*>(p.part_o + (at0 + (size_t)(i + k) * 256 + s * 128) * kPmD + lane * 4);
+        // a share that this row sees nothing of may not have been written; one whose weight comes to 0 is read all the same: a NaN
+        // or infinity in it reaches the row, as it does where one CTA takes all keys
+        if (read) v[k][s] = *reinterpret_cast<const float4*>(p.part_o + (at0 + (size_t)(i + k) * 256 + s * 128) * kPmD + lane * 4);
       }
 #pragma unroll
     for (int k = 0; k < K; ++k)
