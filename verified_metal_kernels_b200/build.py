@@ -70,26 +70,27 @@ def calls_fingerprint():
     return h.hexdigest()
 
 
+def calls_fresh():
+    """Whether _vmk_torch.so is there and was built from what is here now."""
+    if not os.path.exists(CALLS_LIB) or not os.path.exists(CALLS_LIB + ".stamp"):
+        return False
+    with open(CALLS_LIB + ".stamp") as f:
+        return f.read().strip() == calls_fingerprint()
+
+
 def build_calls(force=False):
     """Compile torch_calls.cpp (the kernel modules' ordinary calls, torch tensors to the C entry points) with g++ against
     torch's headers, in-tree.  Returns the path.  Locked and published like the library."""
     import sysconfig
 
     import torch
-    stamp = calls_fingerprint()
-
-    def fresh():
-        if force or not os.path.exists(CALLS_LIB) or not os.path.exists(CALLS_LIB + ".stamp"):
-            return False
-        with open(CALLS_LIB + ".stamp") as f:
-            return f.read().strip() == stamp
-
-    if fresh():
+    if not force and calls_fresh():
         return CALLS_LIB
+    stamp = calls_fingerprint()
     with open(os.path.join(HERE, ".build.lock"), "w") as lock:
         fcntl.flock(lock, fcntl.LOCK_EX)
         try:
-            if not fresh():
+            if force or not calls_fresh():
                 root = os.path.dirname(torch.__file__)
                 tmp = CALLS_LIB + ".tmp.%d" % os.getpid()
                 cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",

@@ -5,7 +5,7 @@ import os
 
 import torch
 
-from .. import _lib
+from .. import _lib, build
 
 _ENTRIES = ("vmk_prompt_workspace_bytes", "vmk_prompt", "vmk_prompt_paged", "vmk_accept", "vmk_pages_workspace_bytes",
             "vmk_pages_reserve", "vmk_pages_append_granted", "vmk_pages_fork", "vmk_pages_compact_granted", "vmk_pages_free", "vmk_pages_copy")
@@ -56,12 +56,16 @@ def elsewhere(dev):
 
 def calls():
     """The compiled form of the modules' ordinary calls (csrc/torch_calls.cpp), loaded on first use.  Its functions return
-    None, having done nothing, for every call that is not ordinary."""
+    None, having done nothing, for every call that is not ordinary.  It reads torch's tensors by the layout of the torch that
+    built it and calls the C entry points by their place in _ENTRIES: one that was built from anything else is not loaded."""
     global _calls
     if _calls is None:
         path = os.path.join(_lib.HERE, "_vmk_torch.so")
         if not os.path.exists(path):
             raise RuntimeError(f"{path} is missing: build it with `python -m verified_metal_kernels_b200.build`")
+        if not build.calls_fresh():
+            raise RuntimeError(f"{path} was built for another torch, Python or source: build it with "
+                               "`python -m verified_metal_kernels_b200.build`")
         lib = _lib.lib()
         spec = importlib.util.spec_from_file_location("_vmk_torch", path)
         module = importlib.util.module_from_spec(spec)
