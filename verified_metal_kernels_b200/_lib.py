@@ -147,11 +147,34 @@ def workspace(nbytes, device, stream_id):
 
 
 def status_word(device):
+    """The status word of a device, made at the first call."""
     import torch
     s = _status.get(device.index)
     if s is None:
-        s = torch.zeros(1, dtype=torch.int32, device=device)
+        with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                s = _status_beside_capture(device)
+            else:
+                s = torch.zeros(1, dtype=torch.int32, device=device)
         _status[device.index] = s
+    return s
+
+
+def _status_beside_capture(device):
+    """Made on the capturing stream, the word would be zeroed at every replay of the graph, whatever other calls had reported.
+    So it is made on a stream of its own, with the thread's capture mode relaxed meanwhile: else a capture forbids the thread to
+    allocate or to wait on any stream."""
+    import torch
+    swap, mode = ctypes.CDLL("libcuda.so.1").cuThreadExchangeStreamCaptureMode, ctypes.c_int(2)
+    if swap(ctypes.byref(mode)) != 0:
+        raise VmkError(-5, "status word: the thread's capture mode cannot be changed")
+    try:
+        side = torch.cuda.Stream(device)
+        with torch.cuda.stream(side):
+            s = torch.zeros(1, dtype=torch.int32, device=device)
+        side.synchronize()
+    finally:
+        swap(ctypes.byref(mode))
     return s
 
 
