@@ -300,8 +300,10 @@ VMK_API int vmk_prompt_paged(const void* q, const void* k_pages, const void* v_p
  * At a node with S = 0, M = 1: child i with token x is accepted iff u[i] M q(x) < r(x) with r = max(p - S q, 0); if not,
  * S += M and M = sum(r) with the new S.  Without draft_probs: accepted iff u[i] M < r(x) with r = p without the tokens
  * refused so far; if not, M -= r(x).  next is the first entry whose cumulative sum of r (of p where r is empty) exceeds
- * u[0] times the whole sum.  All in 64 bits; NaN, infinite and negative entries count as 0; a token outside [0, V) is
- * refused (status). */
+ * u[0] times the whole sum.  Differences are pairs of fp32 numbers, sums fp64: M is off by less
+ * than 2^k (2 n + 3) 2^-47 of the row's sum at a node's k-th refusal (n entries to a thread, V / 512 of a CTA's part of the row),
+ * which is what a decision can be nearer to its border than and still differ from one in exact numbers.  NaN, infinite and
+ * negative entries count as 0; a token outside [0, V) is refused (status). */
 VMK_API int vmk_accept(const void* target_probs, const void* draft_probs, const int32_t* tokens, const uint32_t* bits,
                        int bits_words, const float* u, int32_t* path, int32_t* count, int32_t* next, int B, int kd, int V,
                        int dtype, int32_t* status, void* stream);

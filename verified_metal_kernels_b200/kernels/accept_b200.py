@@ -21,10 +21,10 @@ def kernel(target_probs, tokens, bits, u, draft_probs=None, check=False):
     node's children are tried in ascending order, child i with the number u[:, i]; u[:, 0] draws the next token, from
     what is left of the target where the walk ends.  The tokens that come out are distributed as the target's own.
 
-    path: the accepted nodes in order (path[:, 0] = 0), -1 behind them; count: how many.  Computed in 64 bits.  Entries
-    that are NaN, infinite or negative count as 0; a row of nothing but those gives next_token -1.  A draft token outside
-    [0, V) is refused (and reported in the device status word).  Host tensors are copied in and the results returned on
-    the host."""
+    path: the accepted nodes in order (path[:, 0] = 0), -1 behind them; count: how many.  Differences are
+    pairs of fp32 numbers, sums fp64 (include/vmk_b200.h has the bound of what that is off by).  Entries that are NaN,
+    infinite or negative count as 0; a row of nothing but those gives next_token -1.  A draft token outside [0, V) is refused
+    (and reported in the device status word).  Host tensors are copied in and the results returned on the host."""
     if not check:
         out = calls().accept(target_probs, tokens, bits, u, draft_probs)
         if out is not None:
