@@ -143,6 +143,11 @@ _status = {}
 
 
 def workspace(nbytes, device, stream_id):
+    """Scratch of a call on the current stream of `device`, the current device.  Under stream capture it is the graph's own (from the
+    graph's memory pool): captured graphs neither share it nor lose it to other tensors when a larger one takes its place."""
+    import torch
+    if torch._C._cuda_isCurrentStreamCapturing():
+        return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
     return _workspace.get(nbytes, device, stream_id)
 
 

@@ -83,10 +83,7 @@ def handles(dev):
 
 
 def scratch(nbytes, dev, stream):
-    """Scratch of a call made while `dev` is the current device: address and size.  Under stream capture it is the graph's
-    own (from the graph's memory pool), so that captured graphs do not share it, nor lose it when a larger one takes its place."""
-    if torch._C._cuda_isCurrentStreamCapturing():
-        t = torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
-    else:
-        t = _lib.workspace(nbytes, dev, stream)
+    """Scratch of a call made while `dev` is the current device: address and size.  Its tensor may be let go at once: under
+    capture the graph's memory pool gives it to later calls of the same stream only."""
+    t = _lib.workspace(nbytes, dev, stream)
     return t.data_ptr(), t.numel()
