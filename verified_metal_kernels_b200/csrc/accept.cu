@@ -29,8 +29,8 @@
 // Of a request's kd rows only those are read at which a draft is refused or the walk ends; the rest of the walk needs
 // p and q at (parent, token) of each node, gathered by one thread a node before it begins.  A request is a CLUSTER of
 // up to 8 CTAs that walk its tree in step and split the vocabulary between them: partial sums cross through distributed
-// shared memory.  Measured: 32 trees of 64 nodes over 131072 entries (fp32) 29.7 us, of which the rows that have to be read
-// take 5.2; what bounds it is the chain of passes of the request that is refused most often, each 2.5 to 4 us.  128 chains
+// shared memory.  Measured: 32 trees of 64 nodes over 131072 entries (fp32) 31 us, of which the rows that have to be read
+// take 5.2 (29.7 in a graph, 31 to 34 among other passes); what bounds it is the chain of passes of the request that is refused most often, each 2.5 to 4 us.  128 chains
 // over 100003 entries (bf16) 15 us, one chain of 8 over 32768 entries 6.6 us (latency: two dependent gathers, one pass, the
 // cluster's barrier, one more look at a warp's range).  Inside a CTA every warp owns a contiguous range of the row, so the drawn position is found by prefix
 // over CTAs, then warps, then one warp's range.

@@ -12,10 +12,14 @@
 // the bytes they read and write; those that only keep the tables by latency: one launch each, the giving of pages by ONE
 // CTA (a scan over the counts that stops at the last page needed), so that nothing waits for another CTA.
 //
-// Measured: copying 256 pages of 16 KiB x 8 heads in 8 layers, K and V (1.07 GB moved) 170 us = 6.3 TB/s; 48 rows of up to
-// 1500 positions freed, reserved and filled 55 us = 5.4 TB/s, 128 forks of 32 rows 50 us = 5.6 TB/s; the five launches of
-// one step after a verification (free, reserve, append, compact with its free) 16.3 us, 3 us each.  Letting a launch begin
-// while the one before runs (launch_dependents at the top) made that step 17.7 us.
+// Measured: copying 256 pages of 16 KiB x 8 heads in 8 layers, K and V (1.07 GB moved) 171 us = 6.3 TB/s; 48 rows of up to
+// 1500 positions freed, reserved and filled 56 us = 5.3 TB/s, 128 forks of 32 rows 51 us = 5.5 TB/s; the five launches of
+// one step after a verification (free, reserve, append, compact with its free) 18.3 to 19.7 us.  Before reserve looked at the
+// counts of last pages it was 17.8 on the same GPU (16.3 on another); letting a launch begin while the one before runs
+// (launch_dependents at the top) made those 16.3 17.7.
+//
+// A row grows only into positions of its own: where its last page is partly used and shared, reserve refuses it, and
+// compact moves a row's drafts all together or not at all.
 #include <cstring>
 
 #include "common.cuh"

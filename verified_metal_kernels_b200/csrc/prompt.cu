@@ -31,9 +31,9 @@
 // has completed.  P is rounded to the tensors' 16-bit type before P.V (the tensor pipe takes 16-bit operands); the
 // sum that divides is that of the unrounded P.
 //
-// Measured (bf16, 32 query heads on 8): 32768 tokens 6.6 ms on a cool GPU (1330 TFLOP/s over the visible pairs), 7.4 to 7.7 at
-// the power limit (1.55 to 1.7 GHz); 24 prompts of up to 1999 tokens 247 us; 128 tokens 8.8 us; 17 tokens over 60001 keys 52
-// to 57 us (4.3 to 4.7 TB/s).  What bounds the long ones: each tile's softmax and products follow one another, and two tiles
+// Measured (bf16, 32 query heads on 8): 32768 tokens 6.57 ms at 1.965 GHz (1340 TFLOP/s over the visible pairs), 7.57 at the
+// power limit (1.54 GHz); 24 prompts of up to 1999 tokens 250 us at 1.965 GHz, 287 at 1.64; 128 tokens 8.8 us; 17 tokens over
+// 60001 keys 55 to 58 us (4.2 to 4.5 TB/s).  What bounds the long ones: each tile's softmax and products follow one another, and two tiles
 // keep the tensor pipe and the exponential unit at about 60 % each.  A block of 128 keys costs a pair of tiles 3500 cycles
 // where the products alone take 2060 and the exponentials 2048.  Tried, and slower: scores of 64 keys in two buffers (N = 64
 // products take 48 cycles, not 32), two threads a row, warps of their own for the result, a polynomial for a quarter of the
