@@ -21,17 +21,16 @@
 // only hi is converted and summed in fp64, the brackets are summed in fp32 by each thread (n entries).  So M is off by less
 // than (2 n + 3) 2^-47 of the row's sum, where fp64 throughout is off by some 2^-53, and twice the error of the M before (it
 // is part of S): 2^k (2 n + 3) 2^-47 at the k-th refusal of a node.  Restated in NumPy: below 4e-16 for n of 8 and 256 over five
-// refusals, at an M down to 1e-7.  At the first refusal of a node S is 1 and t is
-// q itself: three subtractions.  A pass over a row that L2 holds is bound by its instructions (20 an element took 4.1 us
+// refusals, at an M down to 1e-7.  At the first refusal of a node S is 1 and t is q itself: three subtractions.  A pass over a row that L2 holds is bound by its instructions (20 an element took 4.1 us
 // for 16384 entries a CTA).  Entries that are NaN, infinite or negative count as 0; a vector that has one is found by one
 // comparison of bits and cleaned in a branch of its own.
 //
 // Of a request's kd rows only those are read at which a draft is refused or the walk ends; the rest of the walk needs
 // p and q at (parent, token) of each node, gathered by one thread a node before it begins.  A request is a CLUSTER of
 // up to 8 CTAs that walk its tree in step and split the vocabulary between them: partial sums cross through distributed
-// shared memory.  Measured: 32 trees of 64 nodes over 131072 entries (fp32) 31 us, of which the rows that have to be read
-// take 5.2 (29.7 in a graph, 31 to 34 among other passes); what bounds it is the chain of passes of the request that is refused most often, each 2.5 to 4 us.  128 chains
-// over 100003 entries (bf16) 15 us, one chain of 8 over 32768 entries 6.6 us (latency: two dependent gathers, one pass, the
+// shared memory.  Measured: 32 trees of 64 nodes over 131072 entries (fp32) 31 to 34 us, of which the rows that
+// have to be read take 5.2; what bounds it is the chain of passes of the request that is refused most often, each 2.5 to 4 us.
+// 128 chains over 100003 entries (bf16) 15 us, one chain of 8 over 32768 entries 6.6 us (latency: two dependent gathers, one pass, the
 // cluster's barrier, one more look at a warp's range).  Inside a CTA every warp owns a contiguous range of the row, so the drawn position is found by prefix
 // over CTAs, then warps, then one warp's range.
 #include <cooperative_groups.h>
